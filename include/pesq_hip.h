@@ -500,6 +500,58 @@ int pesq_epilogue_backward(const float *d_symm, const float *d_asymm, const floa
                            const float *g_loss, int64_t batch, double factor, float *g_symm,
                            float *g_asymm, hipStream_t stream);
 
+/* ----------------------------------------------------------------------- */
+/* operators of the networks that the loss trains                           */
+/* ----------------------------------------------------------------------- */
+
+/* Element types of these operators.  Sums, states and statistics are held in
+ * 32 bits whatever the type, and rounded once where they are written. */
+#define PESQ_F32 0
+#define PESQ_BF16 1
+#define PESQ_F16 2
+
+/* Gated linear recurrence over [batch, time, channels]:
+ *   u = rate softplus(decay) sigmoid(recur_gate),  a = exp(-u)
+ *   h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(input_gate_t) x_t,  y_t = h_t
+ * over rising t, or falling t if `reverse`.  A nonzero reset[b, t] drops the
+ * state before step t (whatever it holds).  `strides` are in elements, per
+ * batch item and per step, of x, recur_gate and input_gate; channels lie next
+ * to each other.  decay [channels], initial [batch, channels] (NULL = 0) and
+ * reset [batch, time] (NULL = none) are contiguous.  At most 65535 batch
+ * items, 2^24 channels and 2^32 steps.  No counterpart in the reference. */
+typedef struct pesq_recurrence {
+    int64_t batch, time, channels;
+    int32_t dtype; /* of x, the gates, y and their gradients */
+    int32_t reverse;
+    double rate; /* > 0 */
+    const void *x, *recur_gate, *input_gate;
+    int64_t strides[3][2];
+    const float *decay;
+    const float *initial;
+    const uint8_t *reset;
+} pesq_recurrence;
+
+/* Bytes of the states that the backward reads (`starts`), and of both passes'
+ * scratch (any may be NULL).  Reads the sizes only. */
+int pesq_recurrence_workspace(const pesq_recurrence *p, size_t *starts, size_t *forward,
+                              size_t *backward);
+
+/* y [batch, time, channels] contiguous, last [batch, channels] (or NULL);
+ * starts may be NULL where no backward follows. */
+int pesq_recurrence_forward(const pesq_recurrence *p, void *y, float *last, float *starts,
+                            void *workspace, hipStream_t stream);
+
+/* Gradients, contiguous, any of them NULL; g_y (g_strides: batch item, step)
+ * and g_last may be NULL, for zero. */
+int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_y, const int64_t *g_strides,
+                             const float *g_last, const float *starts, void *g_x, void *g_recur,
+                             void *g_input, float *g_decay, float *g_initial, void *workspace,
+                             hipStream_t stream);
+
+/* One step (time 1, no reset, `initial` unused) of running streams: state
+ * [batch, channels] is updated in place, y is contiguous. */
+int pesq_recurrence_step(const pesq_recurrence *p, float *state, void *y, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -2,9 +2,9 @@
 
 Every ``csrc/*.hip`` translation unit is compiled by ``hipcc`` into an object
 and linked into one shared library with a plain C ABI (``include/pesq_hip.h``).
-``csrc/torch_autograd.cpp``, the PyTorch autograd node of the fused pipeline,
-is compiled by the host compiler against PyTorch's headers into the extension
-module ``torch_pesq/_lib/_pesq_torch.so``, which links the library.  Both are
+``csrc/torch_autograd.cpp`` and ``csrc/torch_network.cpp``, the PyTorch
+autograd nodes, are compiled by the host compiler against PyTorch's headers into
+the extension module ``torch_pesq/_lib/_pesq_torch.so``, which links the library.  Both are
 built in-tree so that they travel with the source tree.
 """
 
@@ -20,7 +20,7 @@ CSRC = HERE / "csrc"
 OUT_DIR = HERE / "torch_pesq" / "_lib"
 LIB = OUT_DIR / "libpesq_hip.so"
 EXT = OUT_DIR / "_pesq_torch.so"
-EXT_SRC = CSRC / "torch_autograd.cpp"
+EXT_SRCS = [CSRC / "torch_autograd.cpp", CSRC / "torch_network.cpp"]
 OBJ_DIR = HERE / "_build"
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -116,17 +116,17 @@ def build(verbose: bool = False) -> Path:
     OUT_DIR.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
     cflags, ldflags = _torch_flags()
-    ext_obj = OBJ_DIR / (EXT_SRC.stem + ".o")
 
-    def compile_ext():
-        _run([CXX, *cflags, "-c", EXT_SRC, "-o", ext_obj], verbose, f"{CXX} on {EXT_SRC.name}")
-        return ext_obj
+    def compile_ext(src):
+        obj = OBJ_DIR / (src.stem + ".o")
+        _run([CXX, *cflags, "-c", src, "-o", obj], verbose, f"{CXX} on {src.name}")
+        return obj
 
-    workers = min(len(sources) + 1, os.cpu_count() or 1, 8)
+    workers = min(len(sources) + len(EXT_SRCS), os.cpu_count() or 1, 8)
     with ThreadPoolExecutor(max_workers=workers) as pool:
-        ext_job = pool.submit(compile_ext)
+        ext_jobs = [pool.submit(compile_ext, src) for src in EXT_SRCS]
         objects = list(pool.map(lambda s: _compile(s, verbose), sources))
-        ext_job.result()
+        ext_objects = [job.result() for job in ext_jobs]
     tmp = LIB.with_suffix(".so.tmp")
     _run(
         [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-Wl,-soname,libpesq_hip.so",
@@ -136,7 +136,7 @@ def build(verbose: bool = False) -> Path:
     )
     os.replace(tmp, LIB)
     tmp = EXT.with_suffix(".so.tmp")
-    _run([CXX, ext_obj, *ldflags, "-o", tmp], verbose, "linking _pesq_torch.so")
+    _run([CXX, *ext_objects, *ldflags, "-o", tmp], verbose, "linking _pesq_torch.so")
     os.replace(tmp, EXT)
     return LIB
 

@@ -14,50 +14,15 @@
 // exception types first), allocates the outputs and workspaces on the
 // caller's device and enqueues the library calls on PyTorch's current stream.
 
-#include <torch/extension.h>
-
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
 #include <array>
 #include <limits>
 #include <vector>
 #include <stdexcept>
 #include <string>
 
-#include "pesq_hip.h"
+#include "torch_common.hpp"
 
 namespace {
-
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
-
-void check(int status, const char *what) {
-    if (status != PESQ_OK) {
-        throw std::runtime_error(std::string(what) + ": " + pesq_last_error() + " (status " +
-                                 std::to_string(status) + ")");
-    }
-}
-
-hipStream_t current_stream(const at::Tensor &t) {
-    return c10::hip::getCurrentHIPStream(t.get_device()).stream();
-}
-
-template <class T>
-T *data_or_null(const at::Tensor &t) {
-    return t.defined() ? static_cast<T *>(t.data_ptr()) : nullptr;
-}
-
-// Identity whose derivative raises: attached to the gradients when a double
-// backward would need the derivative of the pipeline's backward, as Python's
-// @once_differentiable does.
-struct OnceDifferentiable : public torch::autograd::Function<OnceDifferentiable> {
-    static at::Tensor forward(AutogradContext *, const at::Tensor &x) { return x.clone(); }
-    static variable_list backward(AutogradContext *, variable_list) {
-        throw std::runtime_error(
-            "trying to differentiate twice a function that was marked with @once_differentiable");
-    }
-};
 
 // An STFT geometry other than the pipeline's own (stft undefined: its own): the
 // packed table, frame length and hop.
@@ -980,4 +945,5 @@ PYBIND11_MODULE(_pesq_torch, m) {
         .def("replay", &GraphedStep::replay)
         .def("inputs", &GraphedStep::inputs)
         .def("outputs", &GraphedStep::outputs);
+    bind_network(m);
 }

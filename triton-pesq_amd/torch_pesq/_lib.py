@@ -108,6 +108,27 @@ class ModelConstants(ctypes.Structure):
     ]
 
 
+
+class Recurrence(ctypes.Structure):
+    """``pesq_recurrence``: operands of the gated linear recurrence."""
+
+    _fields_ = [
+        ("batch", ctypes.c_int64),
+        ("time", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reverse", ctypes.c_int32),
+        ("rate", ctypes.c_double),
+        ("x", ctypes.c_void_p),
+        ("recur_gate", ctypes.c_void_p),
+        ("input_gate", ctypes.c_void_p),
+        ("strides", ctypes.c_int64 * 2 * 3),
+        ("decay", ctypes.c_void_p),
+        ("initial", ctypes.c_void_p),
+        ("reset", ctypes.c_void_p),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -213,6 +234,14 @@ SIGNATURES = {
         _INT,
         [_P, _P, _P, _P, _I64, _I64, _I64, ctypes.POINTER(ResamplePlanInfo), _P, _P],
     ),
+    "pesq_recurrence_workspace": (
+        _INT, [ctypes.POINTER(Recurrence), _SIZE_P, _SIZE_P, _SIZE_P],
+    ),
+    "pesq_recurrence_forward": (_INT, [ctypes.POINTER(Recurrence), _P, _P, _P, _P, _P]),
+    "pesq_recurrence_backward": (
+        _INT, [ctypes.POINTER(Recurrence), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "pesq_recurrence_step": (_INT, [ctypes.POINTER(Recurrence), _P, _P, _P]),
 }
 
 _LIB = None
