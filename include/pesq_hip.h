@@ -552,6 +552,72 @@ int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_y, const in
  * [batch, channels] is updated in place, y is contiguous. */
 int pesq_recurrence_step(const pesq_recurrence *p, float *state, void *y, hipStream_t stream);
 
+/* The end of a residual block and the start of the next, over rows of
+ * `channels` neighbours:
+ *   y = branch silu(gate)    x_out = x + scale (y / rms(y)) post_weight
+ *   n_out = x_out / rms(x_out) next_weight        rms(v)^2 = mean(v^2) + eps
+ * gate, scale and next_weight may be NULL (1, 1, no n_out); with branch NULL
+ * (then gate, scale and post_weight too) n_out is of x itself and x_out is not
+ * written.  x, x_out and their gradients have `stream_dtype`, which is `dtype`
+ * or PESQ_F32; all else but the float32 weights has `dtype`.  `strides` are the
+ * rows' of x, branch and gate, in elements; outputs are contiguous.  1 to 8192
+ * channels.  No counterpart in the reference. */
+typedef struct pesq_residual_norm {
+    int64_t rows, channels;
+    int32_t stream_dtype, dtype;
+    double eps;
+    const void *x, *branch, *gate;
+    int64_t strides[3];
+    const float *post_weight, *scale, *next_weight;
+} pesq_residual_norm;
+
+/* Bytes of the backward's scratch. */
+int pesq_residual_norm_workspace(const pesq_residual_norm *p, size_t *backward);
+
+/* `inverse` (1 / rms of y and of x_out, [rows, 2]; or NULL) is what the
+ * backward reads. */
+int pesq_residual_norm_forward(const pesq_residual_norm *p, void *x_out, void *n_out,
+                               float *inverse, hipStream_t stream);
+
+/* Gradients from those of x_out and n_out (either NULL = zero; g_strides: their
+ * rows').  Any output may be NULL, and has to be for an operand that is. */
+int pesq_residual_norm_backward(const pesq_residual_norm *p, const void *g_x_out,
+                                const void *g_n_out, const int64_t *g_strides,
+                                const float *inverse, void *g_x, void *g_branch, void *g_gate,
+                                float *g_post, float *g_scale, float *g_next, void *workspace,
+                                hipStream_t stream);
+
+/* One tensor of an AdamW step.  Its moments are elements first .. first + count
+ * of the moments' arrays; `first` is a multiple of 256. */
+typedef struct pesq_adamw_tensor {
+    void *param;
+    const void *grad;
+    int64_t count;
+    int64_t first;
+} pesq_adamw_tensor;
+
+typedef struct pesq_adamw_options {
+    int32_t dtype;      /* of parameters and gradients */
+    int32_t state_bits; /* 32: float32 moments; 8: int8 and uint8 codes */
+    int64_t step;       /* number of this step, from 1 */
+    double lr, beta1, beta2, eps, weight_decay;
+} pesq_adamw_options;
+
+/* m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2, p = (1 - lr wd) p - lr /
+ * (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps) for every tensor.  With 8 bits
+ * each block of 256 elements of a tensor has one float32 scale per moment, at
+ * first / 256 and on; m = scale q |q| / 127^2 and v = scale q^4 / 255^4.  The
+ * descriptors are read before the call returns.  No counterpart in the
+ * reference. */
+int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
+                    const pesq_adamw_options *options, void *exp_avg, void *exp_avg_sq,
+                    float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream);
+
+/* The values that `count` (a multiple of 256) 8 bit moments stand for. */
+int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float *exp_avg_scale,
+                       const float *exp_avg_sq_scale, int64_t count, float *m, float *v,
+                       hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -208,6 +208,319 @@ at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
     return y;
 }
 
+// ---------------------------------------------------------------------------
+// residual norm
+// ---------------------------------------------------------------------------
+
+// [..., channels] as rows of neighbours: t itself where its rows are evenly spaced
+at::Tensor as_rows(const at::Tensor &t, int64_t rows, int64_t channels) {
+    return dense_rows(t.dim() == 2 ? t : t.reshape({rows, channels}));
+}
+
+struct NormInputs {
+    at::Tensor x, branch, gate, post, scale, next;
+
+    pesq_residual_norm call(double eps) const {
+        pesq_residual_norm p{};
+        const at::Tensor &typed = branch.defined() ? branch : x;
+        p.rows = x.size(0);
+        p.channels = x.size(1);
+        p.stream_dtype = type_code(x, "`x`");
+        p.dtype = type_code(typed, "`branch`");
+        p.eps = eps;
+        const std::array<const at::Tensor *, 3> operands{&x, &branch, &gate};
+        for (int k = 0; k < 3; ++k) {
+            p.strides[k] = operands[k]->defined() ? operands[k]->stride(0) : 0;
+        }
+        p.x = x.data_ptr();
+        p.branch = data(branch);
+        p.gate = data(gate);
+        p.post_weight = data_or_null<float>(post);
+        p.scale = data_or_null<float>(scale);
+        p.next_weight = data_or_null<float>(next);
+        return p;
+    }
+};
+
+struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+    // variables: x, branch, gate, post, scale, next; dtype: of n where there is no branch
+    static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const OptTensor &branch,
+                                 const OptTensor &gate, const OptTensor &post,
+                                 const OptTensor &scale, const OptTensor &next, int64_t dtype,
+                                 double eps, bool keep) {
+        const c10::DeviceGuard guard(x.device());
+        const int64_t channels = x.size(-1), rows = channels ? x.numel() / channels : 0;
+        const auto rows_of = [&](const OptTensor &t) {
+            return t ? as_rows(*t, rows, channels) : at::Tensor();
+        };
+        const auto weight = [](const OptTensor &t) { return t ? t->contiguous() : at::Tensor(); };
+        const NormInputs in{rows_of(x), rows_of(branch), rows_of(gate),
+                            weight(post), weight(scale), weight(next)};
+        pesq_residual_norm p = in.call(eps);
+        if (!branch) p.dtype = static_cast<int32_t>(dtype);
+        const auto of_type = [&](int code) {
+            return x.options().dtype(code == PESQ_F32    ? at::kFloat
+                                     : code == PESQ_BF16 ? at::kBFloat16
+                                                         : at::kHalf);
+        };
+        at::Tensor x_out, n_out, inverse;
+        if (branch) x_out = at::empty(x.sizes(), x.options());
+        if (next) n_out = at::empty(x.sizes(), of_type(p.dtype));
+        if (keep) inverse = at::empty({rows, 2}, x.options().dtype(at::kFloat));
+        check(pesq_residual_norm_forward(&p, data(x_out), data(n_out), data_or_null<float>(inverse),
+                                         current_stream(x)),
+              "pesq_residual_norm_forward");
+        ctx->set_materialize_grads(false);
+        if (keep) {
+            ctx->save_for_backward({in.x, in.branch, in.gate, in.post, in.scale, in.next, inverse});
+            ctx->saved_data["eps"] = eps;
+            ctx->saved_data["dtype"] = static_cast<int64_t>(p.dtype);
+            ctx->saved_data["sizes"] = x.sizes().vec();
+        }
+        variable_list out;
+        if (x_out.defined()) out.push_back(x_out);
+        if (n_out.defined()) out.push_back(n_out);
+        return out;
+    }
+
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        variable_list out(9);
+        const variable_list saved = ctx->get_saved_variables();
+        const NormInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5]};
+        at::Tensor g_x_out, g_n_out;
+        if (in.branch.defined()) g_x_out = grads[0];
+        if (in.next.defined()) g_n_out = grads.back();
+        if (!g_x_out.defined() && !g_n_out.defined()) return out;
+        const c10::DeviceGuard guard(in.x.device());
+        pesq_residual_norm p = in.call(ctx->saved_data["eps"].toDouble());
+        p.dtype = static_cast<int32_t>(ctx->saved_data["dtype"].toInt());
+        const auto sizes = ctx->saved_data["sizes"].toIntVector();
+        {
+            const at::NoGradGuard no_grad;
+            if (g_x_out.defined()) {
+                g_x_out = as_rows(g_x_out.to(in.x.scalar_type()), p.rows, p.channels);
+            }
+            if (g_n_out.defined()) g_n_out = as_rows(g_n_out, p.rows, p.channels);
+        }
+        size_t bytes = 0;
+        check(pesq_residual_norm_workspace(&p, &bytes), "pesq_residual_norm_workspace");
+        at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, in.x.options().dtype(at::kByte));
+        // variables that are there are numbered in order
+        const std::array<const at::Tensor *, 6> operands{&in.x,    &in.branch, &in.gate,
+                                                         &in.post, &in.scale,  &in.next};
+        int variable = 0;
+        for (int k = 0; k < 6; ++k) {
+            if (!operands[k]->defined() || !ctx->needs_input_grad(variable++)) continue;
+            if (k < 3) {
+                out[k] = at::empty(sizes, operands[k]->options());
+            } else {
+                out[k] = at::empty({p.channels}, operands[k]->options());
+            }
+        }
+        at::Tensor g_next = out[5];
+        if (g_next.defined() && !g_n_out.defined()) {
+            g_next.zero_();
+            g_next = at::Tensor();
+        }
+        const std::array<int64_t, 2> strides{g_x_out.defined() ? g_x_out.stride(0) : 0,
+                                             g_n_out.defined() ? g_n_out.stride(0) : 0};
+        check(pesq_residual_norm_backward(
+                  &p, data(g_x_out), data(g_n_out), strides.data(), data_or_null<float>(saved[6]),
+                  data(out[0]), data(out[1]), data(out[2]), data_or_null<float>(out[3]),
+                  data_or_null<float>(out[4]), data_or_null<float>(g_next), data(ws),
+                  current_stream(in.x)),
+              "pesq_residual_norm_backward");
+        mark_once(out, grads);
+        return out;
+    }
+};
+
+void check_weight(const OptTensor &w, const char *name, const at::Tensor &x) {
+    if (!w) return;
+    check_gpu(*w, name, x);
+    TORCH_CHECK(w->is_floating_point() && w->dim() == 1 && w->size(0) == x.size(-1), "`", name,
+                "` has to be a floating [channels] tensor, got ", w->scalar_type(), " ", w->sizes());
+}
+
+// (x, branch, post, gate, scale, next, dtype of n without a branch) -> [x_out][n_out]
+std::vector<at::Tensor> residual_norm(const at::Tensor &x, const OptTensor &branch,
+                                      const OptTensor &post, const OptTensor &gate,
+                                      const OptTensor &scale, const OptTensor &next, double eps,
+                                      std::optional<at::ScalarType> dtype) {
+    TORCH_CHECK(x.is_cuda(), "The HIP backend needs `x` to live on a GPU.");
+    TORCH_CHECK(x.dim() >= 1, "the residual norm expects [..., channels], got a scalar");
+    type_code(x, "`x`");
+    const std::array<std::pair<const char *, const OptTensor *>, 2> rows{
+        {{"branch", &branch}, {"gate", &gate}}};
+    for (const auto &[name, t] : rows) {
+        if (!*t) continue;
+        check_gpu(**t, name, x);
+        TORCH_CHECK((*t)->sizes() == x.sizes(), "`", name, "` has to have the shape of x, ",
+                    x.sizes(), ", got ", (*t)->sizes());
+        type_code(**t, name);
+        TORCH_CHECK((*t)->scalar_type() == branch->scalar_type(), "`gate` has to have the type of "
+                    "the branch, ", branch->scalar_type(), ", got ", (*t)->scalar_type());
+    }
+    int64_t code = 0;
+    const at::ScalarType typed = branch ? branch->scalar_type() : dtype.value_or(x.scalar_type());
+    TORCH_CHECK(x.scalar_type() == at::kFloat || x.scalar_type() == typed, "`x` has to be float32 or "
+                "of the type ", typed, ", got ", x.scalar_type());
+    if (!branch) {
+        TORCH_CHECK(typed == at::kFloat || typed == at::kBFloat16 || typed == at::kHalf,
+                    "the result has to be float32, bfloat16 or float16, got ", typed);
+        code = typed == at::kFloat ? PESQ_F32 : typed == at::kBFloat16 ? PESQ_BF16 : PESQ_F16;
+    }
+    check_weight(post, "weight", x);
+    check_weight(scale, "scale", x);
+    check_weight(next, branch ? "next_weight" : "weight", x);
+    const auto f32 = [](const OptTensor &t) { return t ? OptTensor(t->to(at::kFloat)) : t; };
+    const OptTensor w = f32(post), s = f32(scale), n = f32(next);
+    bool keep = x.requires_grad();
+    for (const OptTensor *t : std::array<const OptTensor *, 5>{&branch, &gate, &w, &s, &n}) {
+        keep = keep || (*t && (*t)->requires_grad());
+    }
+    return ResidualNorm::apply(x, branch, gate, w, s, n, code, eps,
+                               keep && torch::autograd::GradMode::is_enabled());
+}
+
+// ---------------------------------------------------------------------------
+// AdamW
+// ---------------------------------------------------------------------------
+
+// The parameters of one optimizer, the place of each in the moments' arrays,
+// and these arrays.  Gradients are taken from the parameters at each step.
+class AdamWPlan {
+  public:
+    static constexpr int64_t kBlock = 256;
+
+    AdamWPlan(std::vector<std::vector<at::Tensor>> groups, int64_t bits)
+        : groups_(std::move(groups)), bits_(bits) {
+        TORCH_CHECK(bits == 32 || bits == 8, "moments have 32 or 8 bits, got ", bits);
+        at::TensorOptions options;
+        for (const auto &group : groups_) {
+            first_.emplace_back();
+            counts_.emplace_back();
+            for (const at::Tensor &p : group) {
+                TORCH_CHECK(p.is_cuda(), "HipAdamW needs its parameters to live on a GPU.");
+                if (!options.has_device()) options = options.device(p.device());
+                TORCH_CHECK(p.device() == options.device(), "HipAdamW needs all parameters on one GPU.");
+                type_code(p, "a parameter");
+                first_.back().push_back(total_);
+                counts_.back().push_back(p.numel());
+                total_ += (p.numel() + kBlock - 1) / kBlock * kBlock;
+                ++tensors_;
+            }
+        }
+        steps_ = at::zeros({tensors_}, at::kLong);
+        if (tensors_ == 0) return;
+        const auto type = [&](at::ScalarType t) { return options.dtype(t); };
+        if (bits == 32) {
+            arrays_ = {at::zeros({total_}, type(at::kFloat)), at::zeros({total_}, type(at::kFloat))};
+        } else {
+            arrays_ = {at::zeros({total_}, type(at::kChar)), at::zeros({total_}, type(at::kByte)),
+                       at::zeros({total_ / kBlock}, type(at::kFloat)),
+                       at::zeros({total_ / kBlock}, type(at::kFloat))};
+        }
+    }
+
+    // [m, v] or [m, v, scales of m, scales of v] of parameter k of a group, as views
+    std::vector<at::Tensor> views(int64_t group, int64_t k) const {
+        const at::Tensor &p = groups_.at(group).at(k);
+        const int64_t first = first_[group][k], count = counts_[group][k];
+        std::vector<at::Tensor> out;
+        for (size_t n = 0; n < arrays_.size(); ++n) {
+            if (n < 2) {
+                out.push_back(arrays_[n].narrow(0, first, count).view(p.sizes()));
+            } else {
+                out.push_back(arrays_[n].narrow(0, first / kBlock, (count + kBlock - 1) / kBlock));
+            }
+        }
+        return out;
+    }
+
+    at::Tensor steps() const { return steps_; }
+
+    void step(int64_t group, double lr, double beta1, double beta2, double eps,
+              double weight_decay) {
+        struct Bucket {
+            pesq_adamw_options options;
+            std::vector<pesq_adamw_tensor> tensors;
+        };
+        std::vector<Bucket> buckets;  // parameters of one type and step count
+        std::vector<at::Tensor> copies;
+        int64_t at_step = 0;
+        for (int64_t g = 0; g < group; ++g) at_step += static_cast<int64_t>(groups_.at(g).size());
+        int64_t *steps = steps_.data_ptr<int64_t>() + at_step;
+        const auto &params = groups_.at(group);
+        for (size_t k = 0; k < params.size(); ++k) {
+            const at::Tensor &p = params[k];
+            at::Tensor grad = p.grad();
+            if (!grad.defined()) continue;
+            TORCH_CHECK(p.numel() == counts_[group][k] && p.is_contiguous() &&
+                            p.device() == arrays_[0].device(),
+                        "HipAdamW needs contiguous parameters that keep their size and GPU.");
+            TORCH_CHECK(grad.layout() == at::kStrided && grad.scalar_type() == p.scalar_type() &&
+                            grad.sizes() == p.sizes() && grad.device() == p.device(),
+                        "HipAdamW needs dense gradients of the parameters' type and GPU.");
+            if (!grad.is_contiguous()) {
+                grad = grad.contiguous();
+                copies.push_back(grad);
+            }
+            const int32_t dtype = type_code(p, "a parameter");
+            Bucket *bucket = nullptr;
+            for (Bucket &b : buckets) {
+                if (b.options.dtype == dtype && b.options.step == steps[k] + 1) bucket = &b;
+            }
+            if (!bucket) {
+                buckets.push_back({{dtype, static_cast<int32_t>(bits_), steps[k] + 1, lr, beta1, beta2,
+                                    eps, weight_decay}, {}});
+                bucket = &buckets.back();
+                bucket->tensors.reserve(params.size());
+            }
+            bucket->tensors.push_back({p.data_ptr(), grad.data_ptr(), p.numel(), first_[group][k]});
+        }
+        if (buckets.empty()) return;
+        const c10::DeviceGuard guard(arrays_[0].device());
+        const bool eight = bits_ == 8;
+        for (const Bucket &b : buckets) {
+            check(pesq_adamw_step(b.tensors.data(), static_cast<int64_t>(b.tensors.size()), &b.options,
+                                  arrays_[0].data_ptr(), arrays_[1].data_ptr(),
+                                  eight ? arrays_[2].data_ptr<float>() : nullptr,
+                                  eight ? arrays_[3].data_ptr<float>() : nullptr,
+                                  current_stream(arrays_[0])),
+                  "pesq_adamw_step");
+        }
+        for (size_t k = 0; k < params.size(); ++k) {
+            if (!params[k].grad().defined()) continue;
+            ++steps[k];
+            if (!params[k].is_inference()) params[k].unsafeGetTensorImpl()->bump_version();
+        }
+    }
+
+    // [m, v] as float32 arrays: the state's own with 32 bits
+    std::vector<at::Tensor> moments() const {
+        if (bits_ == 32 || arrays_.empty()) return arrays_;
+        const c10::DeviceGuard guard(arrays_[0].device());
+        const auto f32 = arrays_[2].options();
+        std::vector<at::Tensor> out{at::empty({total_}, f32), at::empty({total_}, f32)};
+        check(pesq_adamw_moments(arrays_[0].data_ptr(), arrays_[1].data_ptr(),
+                                 arrays_[2].data_ptr<float>(), arrays_[3].data_ptr<float>(), total_,
+                                 out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+                                 current_stream(arrays_[0])),
+              "pesq_adamw_moments");
+        return out;
+    }
+
+    int64_t first(int64_t group, int64_t k) const { return first_.at(group).at(k); }
+
+  private:
+    std::vector<std::vector<at::Tensor>> groups_;
+    int64_t bits_, total_ = 0, tensors_ = 0;
+    std::vector<std::vector<int64_t>> first_, counts_;
+    at::Tensor steps_;
+    std::vector<at::Tensor> arrays_;
+};
+
 }  // namespace
 
 void bind_network(pybind11::module_ &m) {
@@ -219,4 +532,24 @@ void bind_network(pybind11::module_ &m) {
     m.def("gated_recurrence_step", &gated_recurrence_step,
           "(x, recur_gate, input_gate, decay, state, rate) -> y, the state updated in place",
           arg("x"), arg("recur_gate"), arg("input_gate"), arg("decay"), arg("state"), arg("rate"));
+    m.def(
+        "residual_norm",
+        [](const at::Tensor &x, const OptTensor &branch, const OptTensor &post, const OptTensor &gate,
+           const OptTensor &scale, const OptTensor &next, double eps, const pybind11::object &dtype) {
+            std::optional<at::ScalarType> type;
+            if (!dtype.is_none()) type = torch::python::detail::py_object_to_dtype(dtype);
+            return residual_norm(x, branch, post, gate, scale, next, eps, type);
+        },
+        "(x, branch, weight, gate, scale, next_weight, eps, dtype) -> [x_out][n_out]", arg("x"),
+        arg("branch"), arg("weight"), arg("gate"), arg("scale"), arg("next_weight"), arg("eps"),
+        arg("dtype"));
+    pybind11::class_<AdamWPlan>(m, "AdamWPlan", "the tensors and moments of one optimizer")
+        .def(pybind11::init<std::vector<std::vector<at::Tensor>>, int64_t>(), arg("groups"),
+             arg("bits"))
+        .def("step", &AdamWPlan::step, arg("group"), arg("lr"), arg("beta1"), arg("beta2"),
+             arg("eps"), arg("weight_decay"))
+        .def("views", &AdamWPlan::views)
+        .def("first", &AdamWPlan::first)
+        .def("steps", &AdamWPlan::steps)
+        .def("moments", &AdamWPlan::moments);
 }

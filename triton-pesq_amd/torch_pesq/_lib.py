@@ -129,6 +129,51 @@ class Recurrence(ctypes.Structure):
     ]
 
 
+class ResidualNorm(ctypes.Structure):
+    """``pesq_residual_norm``: operands of the residual norm."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("channels", ctypes.c_int64),
+        ("stream_dtype", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("x", ctypes.c_void_p),
+        ("branch", ctypes.c_void_p),
+        ("gate", ctypes.c_void_p),
+        ("strides", ctypes.c_int64 * 3),
+        ("post_weight", ctypes.c_void_p),
+        ("scale", ctypes.c_void_p),
+        ("next_weight", ctypes.c_void_p),
+    ]
+
+
+class AdamwTensor(ctypes.Structure):
+    """``pesq_adamw_tensor``: one tensor of an AdamW step."""
+
+    _fields_ = [
+        ("param", ctypes.c_void_p),
+        ("grad", ctypes.c_void_p),
+        ("count", ctypes.c_int64),
+        ("first", ctypes.c_int64),
+    ]
+
+
+class AdamwOptions(ctypes.Structure):
+    """``pesq_adamw_options``."""
+
+    _fields_ = [
+        ("dtype", ctypes.c_int32),
+        ("state_bits", ctypes.c_int32),
+        ("step", ctypes.c_int64),
+        ("lr", ctypes.c_double),
+        ("beta1", ctypes.c_double),
+        ("beta2", ctypes.c_double),
+        ("eps", ctypes.c_double),
+        ("weight_decay", ctypes.c_double),
+    ]
+
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _INT = ctypes.c_int
@@ -242,6 +287,16 @@ SIGNATURES = {
         _INT, [ctypes.POINTER(Recurrence), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
     ),
     "pesq_recurrence_step": (_INT, [ctypes.POINTER(Recurrence), _P, _P, _P]),
+    "pesq_residual_norm_workspace": (_INT, [ctypes.POINTER(ResidualNorm), _SIZE_P]),
+    "pesq_residual_norm_forward": (_INT, [ctypes.POINTER(ResidualNorm), _P, _P, _P, _P]),
+    "pesq_residual_norm_backward": (
+        _INT,
+        [ctypes.POINTER(ResidualNorm), _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
+    ),
+    "pesq_adamw_step": (
+        _INT, [ctypes.POINTER(AdamwTensor), _I64, ctypes.POINTER(AdamwOptions), _P, _P, _P, _P, _P],
+    ),
+    "pesq_adamw_moments": (_INT, [_P, _P, _P, _P, _I64, _P, _P, _P]),
 }
 
 _LIB = None
