@@ -91,7 +91,7 @@ def _compare(got, want, dtype, time):
 
 
 SHAPES = [(1, 1, 1), (2, 15, 3), (1, 16, 64), (3, 17, 65), (1, 31, 129), (5, 64, 2), (2, 130, 130), (1, 300, 7),
-          (3, 257, 200), (1, 1025, 33), (1, 4099, 18)]
+          (3, 257, 200), (1, 1025, 33), (1, 4099, 18), (33, 130, 130), (70, 65, 3), (11, 200, 770)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])

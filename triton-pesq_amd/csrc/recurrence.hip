@@ -17,9 +17,10 @@
 // h -> A h + H; parts and chunks are joined by these pairs:
 //
 //   1. each wavefront works its part's pair out, and leaves it in LDS;
-//   2. the first wavefront joins the pairs of the chunk and publishes the
-//      chunk's, then reads those of the chunks before it and folds them, from
-//      the initial state on, into the state at its chunk's start;
+//   2. the pairs of the chunk are joined and published; those of the chunks before
+//      it are read (each wavefront's first look is made with its inputs, so most
+//      have arrived by then) and folded, from the initial state on, into the state
+//      at the chunk's start;
 //   3. each wavefront folds the pairs before its own part onto that state and
 //      runs its steps again, from registers.
 //
@@ -45,13 +46,18 @@
 
 namespace pesq {
 
-constexpr int kSteps = 16;      // steps of a wavefront, and between two kept states
-constexpr int kMaxWaves = 8;    // of a workgroup
-constexpr int kFan = 16;        // chunks whose pairs are joined into one
-constexpr int kBatch = 8;       // pairs read at once
-constexpr int kRecThreads = 64; // of the element-wise kernels
+constexpr int kSteps = 8;           // of a wavefront, and between two kept states
+constexpr int kWaves = 8;           // of a workgroup,
+constexpr int kMaxWaves = 16;       // and of one of a long row
+constexpr int kLongRow = 256;       // chunks of kWaves parts from which a row is long
+constexpr int kFan = 16;            // chunks whose pairs are joined into one
+constexpr int kRound = 16;          // pairs folded between two barriers
+constexpr int kEarly = 2;           // pairs a wavefront looks at with its inputs
+constexpr int kCounters = 64;       // that rows share
+constexpr int kCounterStride = 16;  // words between them: a cache line each
+constexpr int kRecThreads = 64;     // of the element-wise kernels
 constexpr uint64_t kPending = ~uint64_t(0);
-constexpr int kPolls = 1 << 22; // of seconds, far beyond any wait: the result is NaN then
+constexpr int kPolls = 1 << 22;  // seconds, far beyond any wait: the result is NaN then
 
 struct RecArgs {
     int64_t batch, time, channels;
@@ -116,24 +122,59 @@ __device__ __forceinline__ const T *at(const void *p, int64_t b, int64_t sb, int
     return static_cast<const T *>(p) + b * sb + t * st + c;
 }
 
-// V neighbouring channels of type T, as one register: float32 alone, 16 bit
-// types in pairs, or alone where a pair is not aligned
+// V neighbouring channels of type T
 template <class T, int V>
 struct alignas(sizeof(T) * V) Elements {
     T v[V];
 };
 
+// Rows are moved by buffer instructions: one descriptor for a tensor's rows of a
+// part, a uniform offset for the row and one register for the lane's, which is
+// past every buffer's end (reads zeros, writes nothing) for a lane past the
+// row's.
+using Buffer = __amdgpu_buffer_rsrc_t;
+constexpr int kBufferBytes = 0x7fffffff;
+constexpr uint32_t kNoLane = 0x80000000u;
+
+// (none of it is there if p is null)
+__device__ __forceinline__ Buffer buffer_of(const void *p, bool there) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, there ? kBufferBytes : 0, 0x00020000);
+}
+
+// element: the lane's first one, or kNoLane
 template <class T, int V>
-__device__ __forceinline__ Elements<T, V> load_elements(const T *row, int offset) {
-    return *reinterpret_cast<const Elements<T, V> *>(row + offset);
+__device__ __forceinline__ Elements<T, V> load_elements(Buffer buffer, uint32_t element, int row) {
+    using E = Elements<T, V>;
+    const int offset = static_cast<int>(element == kNoLane ? kNoLane : element * sizeof(T));
+    if constexpr (sizeof(E) == 2) {
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(buffer, offset, row, 0));
+    } else if constexpr (sizeof(E) == 4) {
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(buffer, offset, row, 0));
+    } else if constexpr (sizeof(E) == 8) {
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b64(buffer, offset, row, 0));
+    } else {
+        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset, row, 0));
+    }
 }
 
 template <class T, int V>
-__device__ __forceinline__ void store_elements(T *row, int offset, const float (&f)[V]) {
-    Elements<T, V> e;
+__device__ __forceinline__ void store_elements(Buffer buffer, uint32_t element, int row, const float (&f)[V]) {
+    using E = Elements<T, V>;
+    E e;
 #pragma unroll
     for (int k = 0; k < V; ++k) e.v[k] = static_cast<T>(f[k]);
-    *reinterpret_cast<Elements<T, V> *>(row + offset) = e;
+    const int offset = static_cast<int>(element == kNoLane ? kNoLane : element * sizeof(T));
+    if constexpr (sizeof(E) == 2) {
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, e), buffer, offset, row, 0);
+    } else if constexpr (sizeof(E) == 4) {
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), buffer, offset, row, 0);
+    } else if constexpr (sizeof(E) == 8) {
+        typedef uint32_t __attribute__((ext_vector_type(2))) Words;
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Words, e), buffer, offset, row, 0);
+    } else {
+        typedef uint32_t __attribute__((ext_vector_type(4))) Words;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, e), buffer, offset, row, 0);
+    }
 }
 
 // The map h -> a h + b of a stretch of steps.  a is 0 where a reset (or a decay
@@ -151,111 +192,163 @@ __device__ __forceinline__ void publish(uint64_t *word, Pair p) {
                        __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// h mapped by the pairs words[k stride], k = 0 .. count - 1, for V channels,
-// each waited for; with `joined`, the map of all of them too
-template <int V, bool kJoin>
-__device__ __forceinline__ void fold(const uint64_t *words, int64_t count, int64_t stride,
-                                     float (&h)[V], Pair (&joined)[V]) {
-    for (int64_t first = 0; first < count; first += kBatch) {
-        uint64_t got[kBatch][V];
-        bool ready = false;
-        for (int poll = 0; poll < kPolls && !ready; ++poll) {
-            uint64_t all = 0;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-                const int64_t at = first + k < count ? first + k : count - 1;
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    got[k][v] = __hip_atomic_load(words + at * stride + v, __ATOMIC_RELAXED,
-                                                  __HIP_MEMORY_SCOPE_AGENT);
-                }
-            }
-            bool pending = false;
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) pending = pending || got[k][v] == kPending;
-            }
-            ready = !__any(pending);
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            if (first + k >= count) break;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const Pair p{__uint_as_float(static_cast<uint32_t>(got[k][v])),
-                             __uint_as_float(static_cast<uint32_t>(got[k][v] >> 32))};
-                h[v] = p(h[v]);
-                if (kJoin) joined[v] = joined[v].then(p);
-            }
-        }
-    }
-}
-
-// Where a workgroup stands: its chunk in the order of the fold, batch item and
-// channels, and each lane's first channel (of a lane past the end: the last
-// ones, which it reads and does not write).
+// A chunk: its number in the order of the fold, batch item and channels
 struct Place {
-    int64_t chunk, b;
-    int c0, offset;  // first channel of the group; the lane's, after it
-    bool valid;
+    int64_t chunk, row, b;
+    int c0;            // first channel of the group
+    uint32_t element;  // the lane's first, after it, or kNoLane
 };
 
+// LDS of a workgroup: its parts' pairs, those of earlier chunks, and the state
+// before the chunk
 template <int V>
-__device__ __forceinline__ Place place_of(const RecArgs &p, uint32_t ticket, int lane) {
+struct Shared {
+    Pair parts[kMaxWaves][V][kWave];
+    Pair words[kRound][V][kWave];
+    float heads[V][kWave];
+    uint32_t ticket;
+};
+
+__device__ __forceinline__ uint64_t look(const uint64_t *word) {
+    return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// A word once it is there, from the first look at it on
+__device__ __forceinline__ Pair wait_for(const uint64_t *word, uint64_t got) {
+    for (int poll = 0; poll < kPolls && got == kPending; ++poll) got = look(word);
+    return {__uint_as_float(static_cast<uint32_t>(got)), __uint_as_float(static_cast<uint32_t>(got >> 32))};
+}
+
+// A workgroup's chunk: rows (batch items times channel groups) go by the
+// workgroup's number, and the chunk is the next one of the row in the order of
+// the fold, by a counter (from kPending on) of kCounters that rows share.
+template <int V>
+__device__ __forceinline__ Place place_of(const RecArgs &p, uint64_t *words, int lane, Shared<V> &lds) {
     const uint32_t rows = static_cast<uint32_t>(p.batch) * p.groups;
+    const uint32_t lanes = rows < kCounters ? rows : kCounters;
+    // (every lane gets as many workgroups as its rows have chunks)
+    const uint32_t own = blockIdx.x % rows % lanes, count = (rows - own + lanes - 1) / lanes;
+    uint32_t ticket = blockIdx.x / lanes;
+    if (p.chunks > 1) {
+        if (threadIdx.x == 0) {
+            lds.ticket = static_cast<uint32_t>(__hip_atomic_fetch_add(words + own * kCounterStride, uint64_t(1),
+                                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1);
+        }
+        __syncthreads();
+        ticket = lds.ticket;
+    }
+    // (divisions leave uniform values in vector registers)
+    ticket = __builtin_amdgcn_readfirstlane(ticket);
+    const uint32_t chunk = __builtin_amdgcn_readfirstlane(ticket / count);
+    const uint32_t row = own + lanes * (ticket - chunk * count);
+    const int b = __builtin_amdgcn_readfirstlane(static_cast<int>(row / p.groups));
     Place at;
-    at.chunk = ticket / rows;
-    const uint32_t rest = ticket % rows;
-    at.b = rest / p.groups;
-    at.c0 = static_cast<int>(rest % p.groups) * kWave * V;
-    const int left = static_cast<int>(p.channels) - at.c0;
-    at.valid = lane * V < left;
-    at.offset = at.valid ? lane * V : left - V;
+    at.chunk = chunk;
+    at.row = row;
+    at.b = b;
+    at.c0 = __builtin_amdgcn_readfirstlane((static_cast<int>(row) - b * p.groups) * kWave * V);
+    at.element = lane * V < static_cast<int>(p.channels) - at.c0 ? lane * V : kNoLane;
     return at;
 }
 
-// The next chunk in the order of time (words[0] counts them, from kPending on).
-__device__ __forceinline__ uint32_t take_ticket(const RecArgs &p, uint64_t *words) {
-    if (p.chunks == 1) return blockIdx.x;
-    __shared__ uint32_t ticket;
-    if (threadIdx.x == 0) {
-        ticket = static_cast<uint32_t>(__hip_atomic_fetch_add(words, uint64_t(1), __ATOMIC_RELAXED,
-                                                              __HIP_MEMORY_SCOPE_AGENT) + 1);
-    }
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(ticket);
-}
-
-// The state before this chunk from those of the chunks before it (wavefront 0):
-// publishes the chunk's pair, and for every kFan chunks that of all of them.
-// words: [1] pairs [chunks][batch][channels], then joined ones [chunks / kFan].
+// The published pairs of a row: of its chunks, and of kFan chunks each.
+// words: counters, then [chunks][rows][V][64], then [chunks / kFan][rows][V][64]
 template <int V>
-__device__ __forceinline__ void join_chunks(const RecArgs &p, const Place &at, uint64_t *words,
-                                            const Pair (&own)[V], float (&h)[V]) {
-    if (p.chunks == 1) return;
-    const int64_t stride = p.batch * p.channels;
-    uint64_t *pairs = words + 1 + at.b * p.channels + at.c0 + at.offset;
-    uint64_t *joined = pairs + p.chunks * stride;
-    const int64_t fan = at.chunk / kFan, in_fan = at.chunk % kFan;
-    const bool last_of_fan = in_fan == kFan - 1;
-    if (at.valid) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) publish(pairs + at.chunk * stride + v, own[v]);
+struct Published {
+    uint64_t *pairs, *joined;  // of this row and lane
+    int64_t stride;            // to the next chunk's
+    int64_t fan, in_fan;       // joined ones before this chunk, and chunks after them
+    int64_t items, first;      // to fold: in_fan pairs, then the joined ones; of these, in the first round
+
+    __device__ __forceinline__ Published(const RecArgs &p, const Place &at, uint64_t *words, int lane) {
+        stride = p.batch * p.groups * (V * kWave);
+        pairs = words + kCounters * kCounterStride + at.row * (V * kWave) + lane;
+        joined = pairs + p.chunks * stride;
+        fan = p.chunks > 1 ? at.chunk / kFan : 0;
+        in_fan = p.chunks > 1 ? at.chunk % kFan : 0;
+        items = fan + in_fan;
+        // the pairs alone, where others wait for their joined one
+        first = in_fan == kFan - 1 ? in_fan : items < kRound ? items : kRound;
     }
-    Pair all[V];
-    if (last_of_fan) {
-        float none[V] = {};
+    __device__ __forceinline__ const uint64_t *item(int64_t k) const {
+        return k < in_fan ? pairs + (fan * kFan + k) * stride : joined + (k - in_fan) * stride;
+    }
+};
+
+// Each wavefront's first look at a word, together with its inputs: most are there
+template <int V>
+struct Early {
+    uint64_t got[kEarly][V];
+    __device__ __forceinline__ void load(const Published<V> &of, int wave, int waves) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) all[v] = {1.0f, 0.0f};
-        fold<V, true>(pairs + fan * kFan * stride, in_fan, stride, none, all);
-        if (at.valid) {
+        for (int n = 0; n < kEarly; ++n) {
+            const int64_t k = wave + n * waves;
 #pragma unroll
-            for (int v = 0; v < V; ++v) publish(joined + fan * stride + v, all[v].then(own[v]));
+            for (int v = 0; v < V; ++v) got[n][v] = k < of.first ? look(of.item(k) + v * kWave) : kPending;
         }
     }
-    fold<V, false>(joined, fan, stride, h, all);
-    fold<V, false>(pairs + fan * kFan * stride, in_fan, stride, h, all);
+};
+
+// The state before this chunk into lds.heads, from the one before all (initial)
+// and the pairs of the chunks before it; publishes this chunk's pair, and for
+// the last of kFan chunks that of all of them.  The parts' pairs are in LDS; the
+// wavefronts wait for some words each, and wavefront v (all of them, in turn, if
+// there are fewer) folds channel v of each lane.
+template <int V, bool kBack>
+__device__ __forceinline__ void join_chunks(const RecArgs &p, const Place &at, const Published<V> &of,
+                                            const Early<V> &early, int lane, int wave, int waves,
+                                            const Elements<float, V> &initial, Shared<V> &lds) {
+    Pair own[V], near[V];
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (v % waves != wave) continue;
+        h[v] = initial.v[v];
+        near[v] = {1.0f, 0.0f};
+        if (p.chunks == 1) continue;
+        own[v] = lds.parts[kBack ? waves - 1 : 0][v][lane];
+        for (int w = 1; w < waves; ++w) own[v] = own[v].then(lds.parts[kBack ? waves - 1 - w : w][v][lane]);
+        publish(of.pairs + at.chunk * of.stride + v * kWave, own[v]);
+    }
+    for (int64_t first = 0; first < of.items;) {
+        const int64_t left = first == 0 ? of.first : of.items - first;
+        const int here = static_cast<int>(left < kRound ? left : kRound);
+        for (int k = wave, n = 0; k < here; k += waves, ++n) {
+            const uint64_t *word = of.item(first + k);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                uint64_t got = kPending;
+                if (first == 0) {
+#pragma unroll
+                    for (int m = 0; m < kEarly; ++m) got = n == m ? early.got[m][v] : got;
+                }
+                lds.words[k][v][lane] = wait_for(word + v * kWave, got);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (v % waves != wave) continue;
+            for (int k = 0; k < here; ++k) {
+                const Pair q = lds.words[k][v][lane];
+                if (first + k < of.in_fan) {
+                    near[v] = near[v].then(q);
+                } else {
+                    h[v] = q(h[v]);
+                }
+            }
+            if (first == 0 && of.in_fan == kFan - 1) {
+                publish(of.joined + of.fan * of.stride + v * kWave, near[v].then(own[v]));
+            }
+        }
+        first += here;
+        if (first < of.items) __syncthreads();
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        if (v % waves == wave) lds.heads[v][lane] = near[v](h[v]);
+    }
+    __syncthreads();
 }
 
 // bits of the resets of steps n0 ..
@@ -270,95 +363,137 @@ __device__ __forceinline__ uint32_t reset_bits(const RecArgs &p, int64_t b, int6
     return static_cast<uint32_t>(__ballot(set));
 }
 
+// The rows of a wavefront's steps n0 .. n0 + steps - 1 of one tensor, one after
+// another; after the last step, that one again.
+struct Rows {
+    Buffer buffer;
+    int offset, stride, left;  // in bytes; steps still to come after this one
+    __device__ __forceinline__ int next() {
+        const int row = offset;
+        offset += left > 0 ? stride : 0;
+        --left;
+        return row;
+    }
+};
+
+template <class T>
+__device__ __forceinline__ Rows rows_of(const RecArgs &p, const Place &at, int64_t n0, int steps,
+                                        const void *tensor, int64_t sb, int64_t st) {
+    const int64_t t = p.reverse ? p.time - n0 - steps : n0, size = sizeof(T);
+    const int stride = static_cast<int>(st * size);
+    return {buffer_of(static_cast<const char *>(tensor) + (at.b * sb + t * st + at.c0) * size, tensor),
+            p.reverse ? (steps - 1) * stride : 0, p.reverse ? -stride : stride, steps - 1};
+}
+
+// What a wavefront's part of a chunk needs from memory, requested all at once.
+// (steps past the end stand for the last one; none of an empty part)
+template <class T, int V, bool kReset, int kTensors>
+struct Part {
+    Elements<T, V> e[kTensors][kSteps];  // r, i, x and, backward, dy
+    Elements<float, V> decay, start, initial;
+    uint32_t resets;
+    int64_t n0;
+    int left;
+
+    __device__ __forceinline__ void load(const RecArgs &p, const Place &at, int64_t n, int lane, const void *gy,
+                                         int64_t sgb, int64_t sgt, const float *starts, const float *first) {
+        n0 = n;
+        left = n0 >= p.time ? 0 : p.time - n0 < kSteps ? static_cast<int>(p.time - n0) : kSteps;
+        if (left > 0) {
+            Rows r = rows_of<T>(p, at, n0, left, p.r, p.srb, p.srt);
+            Rows i = rows_of<T>(p, at, n0, left, p.i, p.sib, p.sit);
+            Rows x = rows_of<T>(p, at, n0, left, p.x, p.sxb, p.sxt);
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                e[0][s] = load_elements<T, V>(r.buffer, at.element, r.next());
+                e[1][s] = load_elements<T, V>(i.buffer, at.element, i.next());
+                e[2][s] = load_elements<T, V>(x.buffer, at.element, x.next());
+            }
+            if constexpr (kTensors == 4) {
+                Rows g = rows_of<T>(p, at, n0, left, gy, sgb, sgt);
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s) {
+                    e[3][s] = load_elements<T, V>(g.buffer, at.element, g.next());
+                }
+            }
+        }
+        if constexpr (kTensors == 4) {
+            const float *from = starts + (at.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
+            start = load_elements<float, V>(buffer_of(from, left > 0), at.element, 0);
+        }
+        initial = load_elements<float, V>(buffer_of(first + at.b * p.channels + at.c0, first), at.element, 0);
+        decay = load_elements<float, V>(buffer_of(p.decay + at.c0, true), at.element, 0);
+        resets = reset_bits<kReset>(p, at.b, n0, lane);
+    }
+};
+
 template <class T, int V, bool kReset>
 __global__ void __launch_bounds__(kMaxWaves *kWave)
     recurrence_fwd_kernel(RecArgs p, T *y, float *last, float *starts, uint64_t *words) {
-    __shared__ Pair pairs[kMaxWaves][kWave][V];
-    __shared__ float heads[kWave][V];
+    __shared__ Shared<V> lds;
     const int lane = lane_id(), wave = wave_index(), waves = blockDim.x / kWave;
-    const Place at = place_of<V>(p, take_ticket(p, words), lane);
-    const int64_t b = at.b, n0 = (at.chunk * waves + wave) * kSteps;
-    const int64_t channel = at.c0 + at.offset;
-
-    Elements<T, V> rr[kSteps], ri[kSteps], rx[kSteps];
-    const bool some = n0 < p.time;
-    const auto time_of = [&](int s) {
-        const int64_t n = n0 + s < p.time ? n0 + s : p.time - 1;
-        return p.reverse ? p.time - 1 - n : n;
-    };
-    if (some) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int64_t t = time_of(s);
-            rr[s] = load_elements<T, V>(pesq::at<T>(p.r, b, p.srb, t, p.srt, at.c0), at.offset);
-            ri[s] = load_elements<T, V>(pesq::at<T>(p.i, b, p.sib, t, p.sit, at.c0), at.offset);
-            rx[s] = load_elements<T, V>(pesq::at<T>(p.x, b, p.sxb, t, p.sxt, at.c0), at.offset);
-        }
-    }
-    const uint32_t resets = reset_bits<kReset>(p, b, n0, lane);
+    const Place here = place_of<V>(p, words, lane, lds);
+    Part<T, V, kReset, 3> part;
+    part.load(p, here, (here.chunk * waves + wave) * kSteps, lane, nullptr, 0, 0, nullptr, p.initial);
+    const Published<V> of(p, here, words, lane);
+    Early<V> early;
+    early.load(of, wave, waves);
+    __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first wait
+    const int left = part.left;
+    const int64_t n0 = part.n0;
+    const uint32_t resets = part.resets;
     Rate rate[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) rate[v] = channel_rate(p.decay[channel + v], p.rate);
-
-    float a[kSteps][V], in[kSteps][V];
+    float a[kSteps][V], in[kSteps][V], h[V];
     Pair own[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) own[v] = {1.0f, 0.0f};
-    if (some) {
+    for (int v = 0; v < V; ++v) {
+        rate[v] = channel_rate(part.decay.v[v], p.rate);
+        own[v] = {1.0f, 0.0f};
+    }
+    const auto steps = [&](auto full) {
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const bool there = n0 + s < p.time, drop = kReset && (resets >> s & 1);
+            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const Gates g = gates(static_cast<float>(rr[s].v[v]), static_cast<float>(ri[s].v[v]), rate[v]);
+                const Gates g = gates(static_cast<float>(part.e[0][s].v[v]),
+                                      static_cast<float>(part.e[1][s].v[v]), rate[v]);
                 a[s][v] = there ? g.a : 1.0f;
-                in[s][v] = there ? g.s * g.open_i * static_cast<float>(rx[s].v[v]) : 0.0f;
+                in[s][v] = there ? g.s * g.open_i * static_cast<float>(part.e[2][s].v[v]) : 0.0f;
                 own[v].a = drop ? 0.0f : own[v].a * a[s][v];
                 own[v].b = drop ? in[s][v] : fmaf(a[s][v], own[v].b, in[s][v]);
             }
         }
+    };
+    if (left == kSteps) {
+        steps(std::true_type());
+    } else if (left > 0) {
+        steps(std::false_type());
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) pairs[wave][lane][v] = own[v];
+    for (int v = 0; v < V; ++v) lds.parts[wave][v][lane] = own[v];
     __syncthreads();
-    if (wave == 0) {
-        float h[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = p.initial ? p.initial[b * p.channels + channel + v] : 0.0f;
-        Pair chunk[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            chunk[v] = own[v];
-            for (int w = 1; w < waves; ++w) chunk[v] = chunk[v].then(pairs[w][lane][v]);
-        }
-        join_chunks<V>(p, at, words, chunk, h);
-#pragma unroll
-        for (int v = 0; v < V; ++v) heads[lane][v] = h[v];
-    }
-    __syncthreads();
-    float h[V];
+    join_chunks<V, false>(p, here, of, early, lane, wave, waves, part.initial, lds);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        h[v] = heads[lane][v];
-        for (int w = 0; w < wave; ++w) h[v] = pairs[w][lane][v](h[v]);
+        h[v] = lds.heads[v][lane];
+        for (int w = 0; w < wave; ++w) h[v] = lds.parts[w][v][lane](h[v]);
     }
-    if (some && starts && at.valid) {
-        float *out = starts + (b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
-        store_elements<float, V>(out, at.offset, h);
-    }
-    if (some) {
+    if (left > 0) {
+        const float *out = starts + (here.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + here.c0;
+        store_elements<float, V>(buffer_of(out, starts), here.element, 0, h);
+        Rows to = rows_of<T>(p, here, n0, left, y, p.time * p.channels, p.channels);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const bool drop = kReset && (resets >> s & 1);
 #pragma unroll
             for (int v = 0; v < V; ++v) h[v] = drop ? in[s][v] : fmaf(a[s][v], h[v], in[s][v]);
-            if (n0 + s < p.time && at.valid) {
-                store_elements<T, V>(y + (b * p.time + time_of(s)) * p.channels + at.c0, at.offset, h);
-            }
+            // (a step past the end leaves h and writes the last row again)
+            store_elements<T, V>(to.buffer, here.element, to.next(), h);
         }
     }
-    if (last && wave == waves - 1 && at.chunk == p.chunks - 1 && at.valid) {
-        store_elements<float, V>(last + b * p.channels + at.c0, at.offset, h);
+    if (last && wave == waves - 1 && here.chunk == p.chunks - 1) {
+        store_elements<float, V>(buffer_of(last + here.b * p.channels + here.c0, true), here.element, 0, h);
     }
 }
 
@@ -369,100 +504,82 @@ __global__ void __launch_bounds__(kMaxWaves *kWave)
     recurrence_bwd_kernel(RecArgs p, const T *gy, int64_t sgb, int64_t sgt, const float *g_last,
                           const float *starts, T *gx, T *gr, T *gi, float *decay_part,
                           float *g_initial, uint64_t *words) {
-    __shared__ Pair pairs[kMaxWaves][kWave][V];
-    __shared__ float heads[kWave][V];
+    __shared__ Shared<V> lds;
+    __shared__ float sums[kMaxWaves][kWave][V];
     const int lane = lane_id(), wave = wave_index(), waves = blockDim.x / kWave;
-    const Place at = place_of<V>(p, take_ticket(p, words), lane);
-    const int64_t b = at.b, n0 = ((p.chunks - 1 - at.chunk) * waves + wave) * kSteps;
-    const int64_t channel = at.c0 + at.offset;
-
-    Elements<T, V> rr[kSteps], ri[kSteps], rx[kSteps], rg[kSteps];
-    const bool some = n0 < p.time;
-    const auto time_of = [&](int s) {
-        const int64_t n = n0 + s < p.time ? n0 + s : p.time - 1;
-        return p.reverse ? p.time - 1 - n : n;
-    };
-    float h[V];
-    if (some) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int64_t t = time_of(s);
-            rr[s] = load_elements<T, V>(pesq::at<T>(p.r, b, p.srb, t, p.srt, at.c0), at.offset);
-            if (gy) rg[s] = load_elements<T, V>(pesq::at<T>(gy, b, sgb, t, sgt, at.c0), at.offset);
-        }
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int64_t t = time_of(s);
-            ri[s] = load_elements<T, V>(pesq::at<T>(p.i, b, p.sib, t, p.sit, at.c0), at.offset);
-            rx[s] = load_elements<T, V>(pesq::at<T>(p.x, b, p.sxb, t, p.sxt, at.c0), at.offset);
-        }
-        const float *start = starts + (b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
-        const Elements<float, V> held = load_elements<float, V>(start, at.offset);
-#pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = held.v[v];
-    }
-    const uint32_t resets = reset_bits<kReset>(p, b, n0, lane);
+    const Place here = place_of<V>(p, words, lane, lds);
+    Part<T, V, kReset, 4> part;
+    part.load(p, here, ((p.chunks - 1 - here.chunk) * waves + wave) * kSteps, lane, gy, sgb, sgt, starts, g_last);
+    const Published<V> of(p, here, words, lane);
+    Early<V> early;
+    early.load(of, wave, waves);
+    __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first wait
+    const int left = part.left;
+    const int64_t n0 = part.n0;
+    const uint32_t resets = part.resets;
     Rate rate[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) rate[v] = channel_rate(p.decay[channel + v], p.rate);
-
-    float open_r[kSteps][V], a[kSteps][V], g[kSteps][V];
+    float open_r[kSteps][V], a[kSteps][V], g[kSteps][V], c[V], sum[V], h[V];
+    Elements<T, V> ri[kSteps], rx[kSteps];
     Pair own[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) own[v] = {1.0f, 0.0f};
-    if (some) {
+    for (int v = 0; v < V; ++v) {
+        rate[v] = channel_rate(part.decay.v[v], p.rate);
+        h[v] = part.start.v[v];
+        sum[v] = 0.0f;
+        own[v] = {1.0f, 0.0f};
+    }
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        ri[s] = part.e[1][s];
+        rx[s] = part.e[2][s];
+    }
+    const auto towards_start = [&](auto full) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
-            const bool there = n0 + s < p.time, drop = kReset && (resets >> s & 1);
+            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                open_r[s][v] = sigmoid_fast(static_cast<float>(rr[s].v[v]));
+                open_r[s][v] = sigmoid_fast(static_cast<float>(part.e[0][s].v[v]));
                 a[s][v] = exp2_fast(rate[v].k * open_r[s][v]);
-                g[s][v] = gy && there ? static_cast<float>(rg[s].v[v]) : 0.0f;
+                g[s][v] = there ? static_cast<float>(part.e[3][s].v[v]) : 0.0f;
                 const float k = there ? a[s][v] : 1.0f;
                 own[v].a = drop ? 0.0f : own[v].a * k;
                 own[v].b = drop ? 0.0f : k * (g[s][v] + own[v].b);
             }
         }
+    };
+    if (left == kSteps) {
+        towards_start(std::true_type());
+    } else if (left > 0) {
+        towards_start(std::false_type());
     }
 #pragma unroll
-    for (int v = 0; v < V; ++v) pairs[wave][lane][v] = own[v];
+    for (int v = 0; v < V; ++v) lds.parts[wave][v][lane] = own[v];
     __syncthreads();
-    if (wave == 0) {
-        float c[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = g_last ? g_last[b * p.channels + channel + v] : 0.0f;
-        Pair chunk[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            chunk[v] = pairs[waves - 1][lane][v];
-            for (int w = waves - 2; w >= 0; --w) chunk[v] = chunk[v].then(pairs[w][lane][v]);
-        }
-        join_chunks<V>(p, at, words, chunk, c);
-#pragma unroll
-        for (int v = 0; v < V; ++v) heads[lane][v] = c[v];
-    }
-    __syncthreads();
-    float c[V], sum[V];
+    join_chunks<V, true>(p, here, of, early, lane, wave, waves, part.initial, lds);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        sum[v] = 0.0f;
-        c[v] = heads[lane][v];
-        for (int w = waves - 1; w > wave; --w) c[v] = pairs[w][lane][v](c[v]);
+        c[v] = lds.heads[v][lane];
+        for (int w = waves - 1; w > wave; --w) c[v] = lds.parts[w][v][lane](c[v]);
     }
-    if (some) {
+    const auto gradients = [&](auto full) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
-            const bool there = n0 + s < p.time, drop = kReset && (resets >> s & 1);
+            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 g[s][v] += c[v];
                 c[v] = drop ? 0.0f : there ? a[s][v] * g[s][v] : c[v];
             }
         }
+        const int64_t sb = p.time * p.channels;
+        Rows to_x = rows_of<T>(p, here, n0, left, gx, sb, p.channels);
+        Rows to_i = rows_of<T>(p, here, n0, left, gi, sb, p.channels);
+        Rows to_r = rows_of<T>(p, here, n0, left, gr, sb, p.channels);
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
-            const bool there = n0 + s < p.time, drop = kReset && (resets >> s & 1);
+            if (!full.value && s >= left) continue;
+            const bool drop = kReset && (resets >> s & 1);
             float dx[V], dr[V], di[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -471,39 +588,41 @@ __global__ void __launch_bounds__(kMaxWaves *kWave)
                 const float log2a = rate[v].k * open_r[s][v];
                 const float scale = input_scale(log2a, a[s][v]);
                 const float before = drop ? 0.0f : h[v];
-                const float driven = g[s][v] * open_i * x;
-                // a^2 / s is infinite where u is 0; times u (1 - open) it tends to 0
-                const float slope = scale > 0.0f ? a[s][v] * a[s][v] * rcp_fast(scale) : 0.0f;
-                const float du = fmaf(slope, driven, -a[s][v] * before * g[s][v]);
-                dx[v] = g[s][v] * scale * open_i;
-                di[v] = driven * scale * (1.0f - open_i);
+                const float grad = g[s][v], gate = scale * open_i, kept = a[s][v] * before;
+                const float driven = grad * gate * x;
+                // a^2 / s^2 is infinite where u is 0; times s u (1 - open) it tends to 0
+                const float slope = scale > 0.0f ? a[s][v] * a[s][v] * rcp_fast(scale * scale) : 0.0f;
+                const float du = fmaf(slope, driven, -kept * grad);
+                dx[v] = grad * gate;
+                di[v] = fmaf(-driven, open_i, driven);
                 dr[v] = du * (-kLn2 * log2a) * (1.0f - open_r[s][v]);
-                sum[v] += there ? du * open_r[s][v] : 0.0f;
-                h[v] = fmaf(a[s][v], before, scale * open_i * x);
+                sum[v] = fmaf(du, open_r[s][v], sum[v]);
+                h[v] = fmaf(gate, x, kept);
             }
-            if (there && at.valid) {
-                const int64_t row = (b * p.time + time_of(s)) * p.channels + at.c0;
-                if (gx) store_elements<T, V>(gx + row, at.offset, dx);
-                if (gi) store_elements<T, V>(gi + row, at.offset, di);
-                if (gr) store_elements<T, V>(gr + row, at.offset, dr);
-            }
+            store_elements<T, V>(to_x.buffer, here.element, to_x.next(), dx);
+            store_elements<T, V>(to_i.buffer, here.element, to_i.next(), di);
+            store_elements<T, V>(to_r.buffer, here.element, to_r.next(), dr);
         }
+    };
+    if (left == kSteps) {
+        gradients(std::true_type());
+    } else if (left > 0) {
+        gradients(std::false_type());
     }
-    if (g_initial && wave == 0 && at.chunk == p.chunks - 1 && at.valid) {
-        store_elements<float, V>(g_initial + b * p.channels + at.c0, at.offset, c);
+    if (g_initial && wave == 0 && here.chunk == p.chunks - 1) {
+        store_elements<float, V>(buffer_of(g_initial + here.b * p.channels + here.c0, true), here.element, 0, c);
     }
     // the chunk's share of ddecay
-    __shared__ float sums[kMaxWaves][kWave][V];
 #pragma unroll
     for (int v = 0; v < V; ++v) sums[wave][lane][v] = sum[v];
     __syncthreads();
-    if (wave == 0 && at.valid) {
+    if (wave == 0) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             for (int w = 1; w < waves; ++w) sum[v] += sums[w][lane][v];
         }
-        float *out = decay_part + (at.chunk * p.batch + b) * p.channels + at.c0;
-        store_elements<float, V>(out, at.offset, sum);
+        float *out = decay_part + (here.chunk * p.batch + here.b) * p.channels + here.c0;
+        store_elements<float, V>(buffer_of(out, true), here.element, 0, sum);
     }
 }
 
@@ -550,6 +669,9 @@ __global__ void __launch_bounds__(kRecThreads) recurrence_step_kernel(RecArgs p,
 // host side
 // ---------------------------------------------------------------------------
 
+// so that the offsets of a part's rows stay below 2^31 bytes
+constexpr int64_t kMostStride = int64_t(1) << 26;
+
 static int check_recurrence(const pesq_recurrence *p) {
     PESQ_CHECK_ARG(p != nullptr, "null argument");
     PESQ_CHECK_ARG(known_type(p->dtype), "unknown element type %d", int(p->dtype));
@@ -564,6 +686,8 @@ static int check_recurrence(const pesq_recurrence *p) {
     PESQ_CHECK_ARG(p->rate > 0.0 && std::isfinite(p->rate), "the rate has to be positive and finite");
     for (int k = 0; k < 6; ++k) {
         PESQ_CHECK_ARG(p->strides[k / 2][k % 2] >= 0, "negative stride");
+        PESQ_CHECK_ARG(k % 2 == 0 || p->strides[k / 2][1] < kMostStride,
+                       "steps are at most 2^26 elements apart, got %lld", (long long)p->strides[k / 2][1]);
     }
     return PESQ_OK;
 }
@@ -590,10 +714,15 @@ static Plan plan_of(const pesq_recurrence *p, bool paired) {
     plan.v = paired ? 2 : 1;
     plan.groups = cdiv(p->channels, kWave * plan.v);
     const int64_t parts = cdiv(p->time, kSteps);
-    plan.waves = parts < kMaxWaves ? static_cast<int>(parts < 1 ? 1 : parts) : kMaxWaves;
+    // more wavefronts keep the chunks of a long row few: 1 x 64000 x 65 float16 forward
+    // 49 -> 46 us; fewer leave room for two workgroups on a compute unit, one of
+    // which computes while the other waits: 16 x 3751 x 960 bfloat16 201 -> 161 us
+    const int most = parts / kWaves > kLongRow ? kMaxWaves : kWaves;
+    plan.waves = parts < most ? static_cast<int>(parts < 1 ? 1 : parts) : most;
     plan.chunks = parts < 1 ? 1 : cdiv(parts, plan.waves);
     plan.words = plan.chunks == 1 ? 0
-                                  : 1 + (plan.chunks + plan.chunks / kFan) * p->batch * p->channels;
+                                  : kCounters * kCounterStride + (plan.chunks + plan.chunks / kFan) * p->batch *
+                                                                     plan.groups * plan.v * kWave;
     return plan;
 }
 
@@ -664,7 +793,7 @@ extern "C" int pesq_recurrence_workspace(const pesq_recurrence *p, size_t *start
                                          size_t *backward) {
     if (int st = check_recurrence(p)) return st;
     const size_t states = size_t(p->batch) * p->channels * sizeof(float);
-    const Plan plan = plan_of(p, false);  // the same for pairs of channels
+    const Plan plan = plan_of(p, true);  // single channels need no more
     if (starts) *starts = states * cdiv(p->time, kSteps);
     if (forward) *forward = plan.words * sizeof(uint64_t);
     if (backward) *backward = plan.words * sizeof(uint64_t) + states * plan.chunks;
@@ -697,7 +826,7 @@ extern "C" int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_
                                         void *g_input, float *g_decay, float *g_initial,
                                         void *workspace, hipStream_t stream) {
     if (int st = check_operands(p)) return st;
-    PESQ_CHECK_ARG(!g_y || (g_strides && g_strides[0] >= 0 && g_strides[1] >= 0),
+    PESQ_CHECK_ARG(!g_y || (g_strides && g_strides[0] >= 0 && g_strides[1] >= 0 && g_strides[1] < kMostStride),
                    "the upstream gradient needs its strides");
     if (p->channels == 0) return PESQ_OK;
     PESQ_CHECK_ARG(empty(p) || (workspace && (starts || p->time == 0)), "null argument");

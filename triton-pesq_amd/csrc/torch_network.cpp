@@ -105,14 +105,19 @@ void check_state(const at::Tensor &state, const char *name, const at::Tensor &x)
                 state.sizes());
 }
 
+// rows of neighbours, steps as near to each other as the library takes them
+at::Tensor recurrence_rows(const at::Tensor &t) {
+    return t.stride(1) < (int64_t(1) << 26) ? dense_rows(t) : t.contiguous();
+}
+
 struct Recurrence : public torch::autograd::Function<Recurrence> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &recur,
                                  const at::Tensor &input, const at::Tensor &decay,
                                  const OptTensor &initial, const OptTensor &reset, bool reverse,
                                  double rate, bool keep) {
         const c10::DeviceGuard guard(x.device());
-        RecurrenceInputs in{dense_rows(x), dense_rows(recur), dense_rows(input), decay.contiguous(),
-                            initial ? initial->contiguous() : at::Tensor(),
+        RecurrenceInputs in{recurrence_rows(x), recurrence_rows(recur), recurrence_rows(input),
+                            decay.contiguous(), initial ? initial->contiguous() : at::Tensor(),
                             reset ? reset->contiguous() : at::Tensor()};
         const pesq_recurrence p = in.call(reverse, rate);
         size_t starts_bytes = 0, ws_bytes = 0;
@@ -151,7 +156,7 @@ struct Recurrence : public torch::autograd::Function<Recurrence> {
         at::Tensor g_y, g_last;
         {
             const at::NoGradGuard no_grad;
-            if (grads[0].defined()) g_y = dense_rows(grads[0].to(x.scalar_type()));
+            if (grads[0].defined()) g_y = recurrence_rows(grads[0].to(x.scalar_type()));
             if (grads[1].defined()) g_last = grads[1].to(at::kFloat).contiguous();
         }
         for (int k = 0; k < 3; ++k) {
