@@ -608,8 +608,9 @@ typedef struct pesq_adamw_options {
  * (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps) for every tensor.  With 8 bits
  * each block of 256 elements of a tensor has one float32 scale per moment, at
  * first / 256 and on; m = scale q |q| / 127^2 and v = scale q^4 / 255^4.  The
- * descriptors are read before the call returns.  No counterpart in the
- * reference. */
+ * descriptors are read before the call returns.  The moments' arrays start at
+ * multiples of 16 bytes and hold whole blocks, 0 past a tensor's end.  No
+ * counterpart in the reference. */
 int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                     const pesq_adamw_options *options, void *exp_avg, void *exp_avg_sq,
                     float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream);

@@ -33,55 +33,79 @@ struct AdamArgs {
     float b1, c1, b2, c2, keep, step_size, correction, eps;
 };
 
+// A launch takes up to kTensors tensors as kernel arguments: no table to copy to
+// the GPU, and new gradients each step cost nothing.  Workgroups go by tiles of
+// kTile elements; a tile's tensor is found by bisection.
+constexpr int kTensors = 96;
+constexpr int kTileBlocks = 8;  // two for each wavefront
+constexpr int kTile = kTileBlocks * kBlock;
+constexpr int kAdamThreads = 256;
+constexpr int kLane = kBlock / kWave;  // neighbours of a block in a lane
+
+struct AdamTensor {
+    void *param;
+    const void *grad;
+    int64_t count;
+    uint32_t block;  // its first one in the moments
+    uint32_t end;    // number of the tile after its last one
+};
+
+struct AdamList {
+    AdamTensor tensors[kTensors];
+    int count;
+    void *m, *v;
+    float *m_scale, *v_scale;
+    AdamArgs args;
+};
+static_assert(sizeof(AdamList) <= 4096, "kernel arguments");
+
 // as written: no contraction into fused multiply-adds
 #pragma clang fp contract(off)
 
-struct Moments {
-    float m, v;
-};
-
-__device__ __forceinline__ float adamw(float p, float g, Moments &s, const AdamArgs &a) {
-    s.m = s.m * a.b1 + g * a.c1;
-    s.v = s.v * a.b2 + (g * g) * a.c2;
-    const float update = s.m / (sqrtf(s.v) * a.correction + a.eps);
+__device__ __forceinline__ float adamw(float p, float g, float &m, float &v, const AdamArgs &a) {
+    m = m * a.b1 + g * a.c1;
+    v = v * a.b2 + (g * g) * a.c2;
+    const float update = m / (sqrtf(v) * a.correction + a.eps);
     return p * a.keep - update * a.step_size;
 }
 
-__device__ __forceinline__ float value_m(int8_t q, float scale) {
+__device__ __forceinline__ float value_m(int q, float scale) {
     const float part = static_cast<float>(q) * (1.0f / 127.0f);
     return fabsf(part) * part * scale;
 }
 
-__device__ __forceinline__ float value_v(uint8_t q, float scale) {
+__device__ __forceinline__ float value_v(int q, float scale) {
     float part = static_cast<float>(q) * (1.0f / 255.0f);
     part = part * part;
     return part * part * scale;
 }
 
-__device__ __forceinline__ int8_t code_m(float m, float inverse) {
+__device__ __forceinline__ int code_m(float m, float inverse) {
     const float q = rintf(sqrtf(fabsf(m) * inverse) * 127.0f);
     const int code = static_cast<int>(fminf(q, 127.0f));  // fmin: a NaN gives 127
-    return static_cast<int8_t>(m < 0.0f ? -code : code);
+    return m < 0.0f ? -code : code;
 }
 
-__device__ __forceinline__ uint8_t code_v(float v, float inverse) {
+__device__ __forceinline__ int code_v(float v, float inverse) {
     const float q = rintf(sqrtf(sqrtf(v * inverse)) * 255.0f);
     const int code = static_cast<int>(fminf(q, 255.0f));
-    return static_cast<uint8_t>(v > 0.0f && inverse != 0.0f && code < 1 ? 1 : code);
+    return v > 0.0f && inverse != 0.0f && code < 1 ? 1 : code;
 }
 
-// largest magnitude of the block, NaN above all (its bits are the largest)
-__device__ __forceinline__ float block_scale(float v, uint32_t *scratch) {
-    uint32_t bits = __float_as_uint(v) & 0x7fffffffu;
+// largest magnitude of a wavefront's block, NaN above all (its bits are the
+// largest); 0 where it is too small to be held
+__device__ __forceinline__ float block_scale(const float (&f)[kLane]) {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int k = 0; k < kLane; ++k) {
+        const uint32_t other = __float_as_uint(f[k]) & 0x7fffffffu;
+        bits = other > bits ? other : bits;
+    }
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) {
         const uint32_t other = __shfl_xor(bits, m, kWave);
         bits = other > bits ? other : bits;
     }
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) scratch[threadIdx.x / kWave] = bits;
-    __syncthreads();
-    for (int w = 0; w < kBlock / kWave; ++w) bits = scratch[w] > bits ? scratch[w] : bits;
     const float scale = __uint_as_float(bits);
     return scale < kSmallest ? 0.0f : scale;
 }
@@ -89,43 +113,154 @@ __device__ __forceinline__ float block_scale(float v, uint32_t *scratch) {
 __device__ __forceinline__ float inverse_of(float scale) { return scale == 0.0f ? 0.0f : 1.0f / scale; }
 
 template <class T>
-__global__ void __launch_bounds__(kBlock)
-    adamw32_kernel(T *p, const T *g, int64_t count, float *m, float *v, AdamArgs a) {
-    const int64_t k = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-    if (k >= count) return;
-    Moments s{m[k], v[k]};
-    p[k] = static_cast<T>(adamw(static_cast<float>(p[k]), static_cast<float>(g[k]), s, a));
-    m[k] = s.m;
-    v[k] = s.v;
+struct alignas(sizeof(T) * kLane) Lane {
+    T v[kLane];
+};
+
+// a lane's neighbours from element `at` of a tensor; zeros past its end
+template <class T>
+__device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count, bool aligned, float (&out)[kLane]) {
+    if (aligned && at + kLane <= count) {
+        const Lane<T> e = *reinterpret_cast<const Lane<T> *>(p + at);
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) out[k] = static_cast<float>(e.v[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) out[k] = at + k < count ? static_cast<float>(p[at + k]) : 0.0f;
+    }
 }
 
 template <class T>
-__global__ void __launch_bounds__(kBlock)
-    adamw8_kernel(T *p, const T *g, int64_t count, int8_t *m, uint8_t *v, float *m_scale,
-                  float *v_scale, AdamArgs a) {
-    __shared__ uint32_t scratch[kBlock / kWave];
-    const int64_t k = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-    Moments s{0.0f, 0.0f};
-    if (k < count) {
-        s = {value_m(m[k], m_scale[blockIdx.x]), value_v(v[k], v_scale[blockIdx.x])};
-        p[k] = static_cast<T>(adamw(static_cast<float>(p[k]), static_cast<float>(g[k]), s, a));
+__device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, bool aligned, const float (&f)[kLane]) {
+    if (aligned && at + kLane <= count) {
+        Lane<T> e;
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) e.v[k] = static_cast<T>(f[k]);
+        *reinterpret_cast<Lane<T> *>(p + at) = e;
+    } else {
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) {
+            if (at + k < count) p[at + k] = static_cast<T>(f[k]);
+        }
     }
-    const float sm = block_scale(s.m, scratch), sv = block_scale(s.v, scratch);
-    if (threadIdx.x == 0) {
-        m_scale[blockIdx.x] = sm;
-        v_scale[blockIdx.x] = sv;
-    }
-    if (k >= count) return;
-    m[k] = code_m(s.m, inverse_of(sm));
-    v[k] = code_v(s.v, inverse_of(sv));
 }
 
-__global__ void __launch_bounds__(kBlock)
+// The moments' arrays have whole blocks, whose elements past a tensor's end are
+// and stay 0.
+template <class T, bool kEight>
+__global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
+    constexpr int kMine = kTileBlocks / (kAdamThreads / kWave);  // blocks of a wavefront
+    int low = 0, high = list.count - 1;
+    while (low < high) {
+        const int middle = (low + high) / 2;
+        if (blockIdx.x < list.tensors[middle].end) {
+            high = middle;
+        } else {
+            low = middle + 1;
+        }
+    }
+    const AdamTensor &t = list.tensors[low];
+    const uint32_t tile = blockIdx.x - (low ? list.tensors[low - 1].end : 0);
+    const int lane = lane_id();
+    const int64_t count = t.count, block0 = int64_t(tile) * kTileBlocks + wave_index() * kMine;
+    T *param = static_cast<T *>(t.param);
+    const T *grad = static_cast<const T *>(t.grad);
+    const bool aligned = (reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) % sizeof(Lane<T>) == 0;
+    const AdamArgs a = list.args;
+
+    float p[kMine][kLane], g[kMine][kLane], m[kMine][kLane], v[kMine][kLane];
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+        const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
+        if (block * kBlock >= count) break;
+        load_lane(param, at, count, aligned, p[n]);
+        load_lane(grad, at, count, aligned, g[n]);
+        const int64_t held = int64_t(t.block) + block;
+        if constexpr (kEight) {
+            const Lane<int8_t> cm = static_cast<const Lane<int8_t> *>(list.m)[held * kWave + lane];
+            const Lane<uint8_t> cv = static_cast<const Lane<uint8_t> *>(list.v)[held * kWave + lane];
+            const float sm = list.m_scale[held], sv = list.v_scale[held];
+#pragma unroll
+            for (int k = 0; k < kLane; ++k) {
+                m[n][k] = value_m(cm.v[k], sm);
+                v[n][k] = value_v(cv.v[k], sv);
+            }
+        } else {
+            const Lane<float> em = static_cast<const Lane<float> *>(list.m)[held * kWave + lane];
+            const Lane<float> ev = static_cast<const Lane<float> *>(list.v)[held * kWave + lane];
+#pragma unroll
+            for (int k = 0; k < kLane; ++k) {
+                m[n][k] = em.v[k];
+                v[n][k] = ev.v[k];
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < kMine; ++n) {
+        const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
+        if (block * kBlock >= count) break;
+#pragma unroll
+        for (int k = 0; k < kLane; ++k) p[n][k] = adamw(p[n][k], g[n][k], m[n][k], v[n][k], a);
+        store_lane(param, at, count, aligned, p[n]);
+        const int64_t held = int64_t(t.block) + block;
+        if constexpr (kEight) {
+            const float sm = block_scale(m[n]), sv = block_scale(v[n]);
+            const float im = inverse_of(sm), iv = inverse_of(sv);
+            Lane<int8_t> cm;
+            Lane<uint8_t> cv;
+#pragma unroll
+            for (int k = 0; k < kLane; ++k) {
+                cm.v[k] = static_cast<int8_t>(at + k < count ? code_m(m[n][k], im) : 0);
+                cv.v[k] = static_cast<uint8_t>(at + k < count ? code_v(v[n][k], iv) : 0);
+            }
+            static_cast<Lane<int8_t> *>(list.m)[held * kWave + lane] = cm;
+            static_cast<Lane<uint8_t> *>(list.v)[held * kWave + lane] = cv;
+            if (lane == 0) {
+                list.m_scale[held] = sm;
+                list.v_scale[held] = sv;
+            }
+        } else {
+            Lane<float> em, ev;
+#pragma unroll
+            for (int k = 0; k < kLane; ++k) {
+                em.v[k] = m[n][k];
+                ev.v[k] = v[n][k];
+            }
+            static_cast<Lane<float> *>(list.m)[held * kWave + lane] = em;
+            static_cast<Lane<float> *>(list.v)[held * kWave + lane] = ev;
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kAdamThreads)
     adamw_moments_kernel(const int8_t *m, const uint8_t *v, const float *m_scale,
-                         const float *v_scale, float *m_out, float *v_out) {
-    const int64_t k = int64_t(blockIdx.x) * kBlock + threadIdx.x;
-    m_out[k] = value_m(m[k], m_scale[blockIdx.x]);
-    v_out[k] = value_v(v[k], v_scale[blockIdx.x]);
+                         const float *v_scale, int64_t blocks, float *m_out, float *v_out) {
+    const int64_t block = int64_t(blockIdx.x) * (kAdamThreads / kWave) + wave_index();
+    if (block >= blocks) return;
+    const int64_t at = block * kWave + lane_id();
+    const Lane<int8_t> cm = reinterpret_cast<const Lane<int8_t> *>(m)[at];
+    const Lane<uint8_t> cv = reinterpret_cast<const Lane<uint8_t> *>(v)[at];
+    const float sm = m_scale[block], sv = v_scale[block];
+    Lane<float> em, ev;
+#pragma unroll
+    for (int k = 0; k < kLane; ++k) {
+        em.v[k] = value_m(cm.v[k], sm);
+        ev.v[k] = value_v(cv.v[k], sv);
+    }
+    reinterpret_cast<Lane<float> *>(m_out)[at] = em;
+    reinterpret_cast<Lane<float> *>(v_out)[at] = ev;
+}
+
+// the launch of a list of `tiles` tiles
+static void launch_adamw(const AdamList &list, int dtype, bool eight, uint32_t tiles, hipStream_t stream) {
+    with_type(dtype, [&](auto type) {
+        using T = decltype(type);
+        if (eight) {
+            adamw_kernel<T, true><<<tiles, kAdamThreads, 0, stream>>>(list);
+        } else {
+            adamw_kernel<T, false><<<tiles, kAdamThreads, 0, stream>>>(list);
+        }
+    });
 }
 
 }  // namespace pesq
@@ -135,6 +270,7 @@ using namespace pesq;
 extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                                const pesq_adamw_options *o, void *exp_avg, void *exp_avg_sq,
                                float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
+    constexpr int64_t kMostTiles = int64_t(1) << 30;
     PESQ_CHECK_ARG(o != nullptr && count >= 0 && (tensors || count == 0), "null argument");
     PESQ_CHECK_ARG(known_type(o->dtype), "unknown element type %d", int(o->dtype));
     PESQ_CHECK_ARG(o->state_bits == 32 || o->state_bits == 8, "moments have 32 or 8 bits, got %d",
@@ -145,11 +281,15 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
     const bool eight = o->state_bits == 8;
     PESQ_CHECK_ARG(count == 0 || (exp_avg && exp_avg_sq && (!eight || (exp_avg_scale && exp_avg_sq_scale))),
                    "null argument");
+    for (const void *array : {exp_avg, exp_avg_sq}) {
+        PESQ_CHECK_ARG(reinterpret_cast<uintptr_t>(array) % 16 == 0, "the moments start at multiples of 16 bytes");
+    }
     for (int64_t k = 0; k < count; ++k) {
         PESQ_CHECK_ARG(tensors[k].count >= 0 && tensors[k].first >= 0 && tensors[k].first % kBlock == 0,
                        "tensor %lld has no place in the moments", (long long)k);
         PESQ_CHECK_ARG(tensors[k].count == 0 || (tensors[k].param && tensors[k].grad), "null argument");
-        PESQ_CHECK_ARG(tensors[k].count < (int64_t(1) << 39), "tensor %lld is too large", (long long)k);
+        PESQ_CHECK_ARG(tensors[k].count <= kMostTiles * kTile && tensors[k].first < (int64_t(1) << 40),
+                       "tensor %lld is too large", (long long)k);
     }
     const double step = static_cast<double>(o->step);
     const AdamArgs a{static_cast<float>(o->beta1), static_cast<float>(1.0 - o->beta1),
@@ -158,25 +298,30 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                      static_cast<float>(o->lr / (1.0 - std::pow(o->beta1, step))),
                      static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(o->beta2, step))),
                      static_cast<float>(o->eps)};
+    AdamList list;
+    list.count = 0;
+    list.m = exp_avg;
+    list.v = exp_avg_sq;
+    list.m_scale = exp_avg_scale;
+    list.v_scale = exp_avg_sq_scale;
+    list.args = a;
+    int64_t tiles = 0;
     for (int64_t k = 0; k < count; ++k) {
         const pesq_adamw_tensor &t = tensors[k];
         if (t.count == 0) continue;
-        const unsigned grid = static_cast<unsigned>(cdiv(t.count, kBlock));
-        with_type(o->dtype, [&](auto type) {
-            using T = decltype(type);
-            if (eight) {
-                adamw8_kernel<T><<<grid, kBlock, 0, stream>>>(
-                    static_cast<T *>(t.param), static_cast<const T *>(t.grad), t.count,
-                    static_cast<int8_t *>(exp_avg) + t.first,
-                    static_cast<uint8_t *>(exp_avg_sq) + t.first, exp_avg_scale + t.first / kBlock,
-                    exp_avg_sq_scale + t.first / kBlock, a);
-            } else {
-                adamw32_kernel<T><<<grid, kBlock, 0, stream>>>(
-                    static_cast<T *>(t.param), static_cast<const T *>(t.grad), t.count,
-                    static_cast<float *>(exp_avg) + t.first,
-                    static_cast<float *>(exp_avg_sq) + t.first, a);
-            }
-        });
+        const int64_t more = cdiv(t.count, kTile);
+        if (list.count == kTensors || tiles + more > kMostTiles) {
+            launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
+            PESQ_CHECK_LAUNCH("pesq_adamw_step");
+            list.count = 0;
+            tiles = 0;
+        }
+        tiles += more;
+        list.tensors[list.count++] = {t.param, t.grad, t.count, static_cast<uint32_t>(t.first / kBlock),
+                                      static_cast<uint32_t>(tiles)};
+    }
+    if (list.count > 0) {
+        launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
         PESQ_CHECK_LAUNCH("pesq_adamw_step");
     }
     return PESQ_OK;
@@ -189,9 +334,13 @@ extern "C" int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq,
                    "whole blocks of %d elements, got %lld", kBlock, (long long)count);
     if (count == 0) return PESQ_OK;
     PESQ_CHECK_ARG(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && m && v, "null argument");
-    adamw_moments_kernel<<<static_cast<unsigned>(count / kBlock), kBlock, 0, stream>>>(
+    for (const void *array : {exp_avg, exp_avg_sq, static_cast<const void *>(m), static_cast<const void *>(v)}) {
+        PESQ_CHECK_ARG(reinterpret_cast<uintptr_t>(array) % 16 == 0, "the moments start at multiples of 16 bytes");
+    }
+    const int64_t blocks = count / kBlock;
+    adamw_moments_kernel<<<static_cast<unsigned>(cdiv(blocks, kAdamThreads / kWave)), kAdamThreads, 0, stream>>>(
         static_cast<const int8_t *>(exp_avg), static_cast<const uint8_t *>(exp_avg_sq), exp_avg_scale,
-        exp_avg_sq_scale, m, v);
+        exp_avg_sq_scale, blocks, m, v);
     PESQ_CHECK_LAUNCH("pesq_adamw_moments");
     return PESQ_OK;
 }
