@@ -80,16 +80,44 @@ __device__ __forceinline__ float value_v(int q, float scale) {
     return part * part * scale;
 }
 
-__device__ __forceinline__ int code_m(float m, float inverse) {
-    const float q = rintf(sqrtf(fabsf(m) * inverse) * 127.0f);
-    const int code = static_cast<int>(fminf(q, 127.0f));  // fmin: a NaN gives 127
-    return m < 0.0f ? -code : code;
+template <class T>
+struct alignas(sizeof(T) * kLane) Lane {
+    T v[kLane];
+};
+
+// Codes are those of correctly rounded roots.  The hardware's root (one unit in
+// the last place) gives the same code unless the product lies next to the middle
+// between two: within 127 2^-22 of it for the first moment and 255 2^-22 for the
+// second's two roots, twice the errors that can arise.  A block with such an
+// element, one in twenty, is done again.
+__device__ __forceinline__ bool near_middle(float q, float distance) {
+    return fabsf(fabsf(q - rintf(q)) - 0.5f) <= distance;
 }
 
-__device__ __forceinline__ int code_v(float v, float inverse) {
-    const float q = rintf(sqrtf(sqrtf(v * inverse)) * 255.0f);
-    const int code = static_cast<int>(fminf(q, 255.0f));
-    return v > 0.0f && inverse != 0.0f && code < 1 ? 1 : code;
+template <bool kExact>
+__device__ __forceinline__ bool codes(const float (&m)[kLane], const float (&v)[kLane], float im, float iv,
+                                      Lane<int8_t> &cm, Lane<uint8_t> &cv) {
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < kLane; ++k) {
+        const float ym = fabsf(m[k]) * im, yv = v[k] * iv;
+        const float qm = (kExact ? sqrtf(ym) : __builtin_amdgcn_sqrtf(ym)) * 127.0f;
+        const float qv =
+            (kExact ? sqrtf(sqrtf(yv)) : __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(yv))) * 255.0f;
+        if (!kExact) near = near || near_middle(qm, 127.0f * 0x1p-22f) || near_middle(qv, 255.0f * 0x1p-22f);
+        const int code = static_cast<int>(fminf(rintf(qm), 127.0f));  // fmin: a NaN gives 127
+        cm.v[k] = static_cast<int8_t>(m[k] < 0.0f ? -code : code);
+        const int root = static_cast<int>(fminf(rintf(qv), 255.0f));
+        cv.v[k] = static_cast<uint8_t>(v[k] > 0.0f && iv != 0.0f && root < 1 ? 1 : root);
+    }
+    return near;
+}
+
+template <int kCtrl>
+__device__ __forceinline__ uint32_t max_ror(uint32_t v) {
+    const uint32_t other = static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(v), kCtrl, 0xF, 0xF, true));
+    return other > v ? other : v;
 }
 
 // largest magnitude of a wavefront's block, NaN above all (its bits are the
@@ -101,21 +129,20 @@ __device__ __forceinline__ float block_scale(const float (&f)[kLane]) {
         const uint32_t other = __float_as_uint(f[k]) & 0x7fffffffu;
         bits = other > bits ? other : bits;
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        const uint32_t other = __shfl_xor(bits, m, kWave);
-        bits = other > bits ? other : bits;
-    }
+    bits = max_ror<0x128>(bits);  // row_ror:8, 4, 2, 1
+    bits = max_ror<0x124>(bits);
+    bits = max_ror<0x122>(bits);
+    bits = max_ror<0x121>(bits);
+    const auto row = [&](int lane) {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits), lane));
+    };
+    const uint32_t low = row(0) > row(16) ? row(0) : row(16), high = row(32) > row(48) ? row(32) : row(48);
+    bits = low > high ? low : high;
     const float scale = __uint_as_float(bits);
     return scale < kSmallest ? 0.0f : scale;
 }
 
 __device__ __forceinline__ float inverse_of(float scale) { return scale == 0.0f ? 0.0f : 1.0f / scale; }
-
-template <class T>
-struct alignas(sizeof(T) * kLane) Lane {
-    T v[kLane];
-};
 
 // a lane's neighbours from element `at` of a tensor; zeros past its end
 template <class T>
@@ -199,6 +226,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     for (int n = 0; n < kMine; ++n) {
         const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
         if (block * kBlock >= count) break;
+        // (past the end m, v and g are 0, and the moments stay 0)
 #pragma unroll
         for (int k = 0; k < kLane; ++k) p[n][k] = adamw(p[n][k], g[n][k], m[n][k], v[n][k], a);
         store_lane(param, at, count, aligned, p[n]);
@@ -208,11 +236,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
             const float im = inverse_of(sm), iv = inverse_of(sv);
             Lane<int8_t> cm;
             Lane<uint8_t> cv;
-#pragma unroll
-            for (int k = 0; k < kLane; ++k) {
-                cm.v[k] = static_cast<int8_t>(at + k < count ? code_m(m[n][k], im) : 0);
-                cv.v[k] = static_cast<uint8_t>(at + k < count ? code_v(v[n][k], iv) : 0);
-            }
+            if (__any(codes<false>(m[n], v[n], im, iv, cm, cv))) codes<true>(m[n], v[n], im, iv, cm, cv);
             static_cast<Lane<int8_t> *>(list.m)[held * kWave + lane] = cm;
             static_cast<Lane<uint8_t> *>(list.v)[held * kWave + lane] = cv;
             if (lane == 0) {
