@@ -90,10 +90,11 @@ def _plain_values(q, scale, signed):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-def test_8_bit_steps_match_the_plain_form_bit_for_bit(dtype):
+def test_8_bit_moments_match_the_plain_form_bit_for_bit(dtype):
     params = _params(dtype, seed=1)
     opt = HipAdamW(params, lr=2e-3, state_bits=8)
     plain = [p.detach().clone() for p in params]
+    sizes = [None] * len(params)
     held = [(_plain_codes(torch.zeros(p.shape, device="cuda"), True),
              _plain_codes(torch.zeros(p.shape, device="cuda"), False)) for p in params]
     for step in range(1, 6):
@@ -107,12 +108,16 @@ def test_8_bit_steps_match_the_plain_form_bit_for_bit(dtype):
             v = _plain_values(*held[k][1], False) * 0.999 + (g * g) * (1.0 - 0.999)
             update = m / (torch.sqrt(v) * correction + 1e-8)
             plain[k] = (plain[k].float() * (1.0 - 2e-3 * 0.01) - update * step_size).to(dtype)
+            sizes[k] = (update * step_size).double().abs()
             held[k] = (_plain_codes(m, True), _plain_codes(v, False))
         opt.step()
         flat = opt.moments()
         for k, p in enumerate(params):
             state = opt.state[p]
-            assert torch.equal(p.detach(), plain[k]), (step, k)
+            # the step's quotient is four units off at most, and p rounded once
+            off = (p.detach().double() - plain[k].double()).abs()
+            assert (off <= 4 * 2.0**-23 * sizes[k] + (2.0**-23 + 2 * HALF_UNIT[dtype]) * plain[k].double().abs()).all(), (step, k)
+            plain[k] = p.detach().clone()
             for name, (q, scale), signed in (("exp_avg", held[k][0], True), ("exp_avg_sq", held[k][1], False)):
                 assert torch.equal(state[name], q), (step, k, name)
                 assert torch.equal(state[name + "_scale"], scale), (step, k, name)
@@ -180,6 +185,22 @@ def test_zero_tiny_and_non_finite_gradients():
             state = opt.state[params[2]]
             assert not torch.isfinite(state["exp_avg_scale"][:2]).any()
             assert torch.isfinite(state["exp_avg_scale"][2:]).all() and torch.isfinite(m[512:]).all()
+
+
+def test_without_eps():
+    """eps = 0: no update where the moments are zero, a full one where the second
+    moment is far below what its square can hold in float32."""
+
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(600, device="cuda"))
+        opt = HipAdamW([p], lr=1e-2, eps=0.0, weight_decay=0.0, state_bits=bits)
+        p.grad = torch.zeros_like(p)
+        p.grad[300:] = 1e-3
+        p.grad[400:] = 1e-25
+        opt.step()
+        assert (p[:300] == 1).all() and torch.isfinite(p).all()
+        assert torch.allclose(p[300:400], torch.full((100,), 0.99, device="cuda"), rtol=1e-5)
+        assert ((p[400:] > 0.98) & (p[400:] <= 1)).all()
 
 
 def test_groups_missing_gradients_and_step_counts():
