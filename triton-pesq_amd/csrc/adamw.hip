@@ -214,7 +214,8 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     const int64_t count = t.count, block0 = int64_t(tile) * kTileBlocks + wave_index() * kMine;
     T *param = static_cast<T *>(t.param);
     const T *grad = static_cast<const T *>(t.grad);
-    const bool aligned = (reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) % sizeof(Lane<T>) == 0;
+    const bool aligned =
+        (reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) % sizeof(Lane<T>) == 0;
     const AdamArgs a = list.args;
 
     float p[kMine][kLane], g[kMine][kLane], m[kMine][kLane], v[kMine][kLane];
@@ -303,7 +304,7 @@ using namespace pesq;
 extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                                const pesq_adamw_options *o, void *exp_avg, void *exp_avg_sq,
                                float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
-    constexpr int64_t kMostTiles = int64_t(1) << 30;
+    constexpr int64_t kMostTiles = (int64_t(1) << 32) / kAdamThreads - 1;  // of a launch
     PESQ_CHECK_ARG(o != nullptr && count >= 0 && (tensors || count == 0), "null argument");
     PESQ_CHECK_ARG(known_type(o->dtype), "unknown element type %d", int(o->dtype));
     PESQ_CHECK_ARG(o->state_bits == 32 || o->state_bits == 8, "moments have 32 or 8 bits, got %d",
@@ -363,8 +364,8 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
 extern "C" int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq,
                                   const float *exp_avg_scale, const float *exp_avg_sq_scale,
                                   int64_t count, float *m, float *v, hipStream_t stream) {
-    PESQ_CHECK_ARG(count >= 0 && count % kBlock == 0 && count < (int64_t(1) << 39),
-                   "whole blocks of %d elements, got %lld", kBlock, (long long)count);
+    PESQ_CHECK_ARG(count >= 0 && count % kBlock == 0 && count < (int64_t(1) << 34),
+                   "whole blocks of %d elements, 2^34 elements at most, got %lld", kBlock, (long long)count);
     if (count == 0) return PESQ_OK;
     PESQ_CHECK_ARG(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && m && v, "null argument");
     for (const void *array : {exp_avg, exp_avg_sq, static_cast<const void *>(m), static_cast<const void *>(v)}) {

@@ -10,8 +10,8 @@
 //   dr_t = du_t u_t (1 - sigmoid(r_t))
 //   ddecay = rate sigmoid(decay) sum_t du_t sigmoid(r_t)          dh_0 = a_1 G_1
 //
-// One pass over the data.  A wavefront takes kSteps steps of 64 (or 128, two a
-// lane) channels and holds them in registers; the wavefronts of a workgroup take
+// One pass over the data.  A wavefront takes kSteps steps of 64 channels and holds
+// them in registers; the wavefronts of a workgroup take
 // consecutive parts of a chunk of time, and the chunks of one row are separate
 // workgroups.  A part maps the state before it to the state after it by
 // h -> A h + H; parts and chunks are joined by these pairs:
@@ -46,10 +46,10 @@
 
 namespace pesq {
 
-constexpr int kSteps = 8;           // of a wavefront, and between two kept states
-constexpr int kWaves = 8;           // of a workgroup,
+constexpr int kSteps = 16;          // of a wavefront, and between two kept states
+constexpr int kWaves = 4;           // of a workgroup,
 constexpr int kMaxWaves = 16;       // and of one of a long row
-constexpr int kLongRow = 256;       // chunks of kWaves parts from which a row is long
+constexpr int kLongRow = 256;       // chunks of kWaves parts that a row has at most, or is long
 constexpr int kFan = 16;            // chunks whose pairs are joined into one
 constexpr int kRound = 16;          // pairs folded between two barriers
 constexpr int kEarly = 2;           // pairs a wavefront looks at with its inputs
@@ -68,21 +68,35 @@ struct RecArgs {
     float rate;
     bool reverse;
     int64_t chunks;  // per row
-    int32_t groups;  // of 64 (or 128) channels
+    int32_t groups;  // of 64 channels
+    const float *rates;  // open_log2 of every channel, or NULL
 };
 
-struct Rate {
-    float k;       // log2 of the decay at an open gate, <= 0
-    float factor;  // d u / d decay at an open gate: rate sigmoid(decay)
-};
-
-// rate softplus(decay), the logarithm of 1 + y as y log(w) / (w - 1), w = 1 + y
-// rounded, which is exact where y is small
-__device__ __forceinline__ Rate channel_rate(float decay, float rate) {
-    const float y = exp2_fast(-kLog2e * fabsf(decay));
-    const float w = 1.0f + y;
-    const float log1p = w == 1.0f ? y : kLn2 * log2_fast(w) * y * rcp_fast(w - 1.0f);
-    return {-(fmaxf(decay, 0.0f) + log1p) * rate * kLog2e, rate * sigmoid_fast(decay)};
+// log2 of a channel's a at an open gate, -rate softplus(decay) log2(e) <= 0, to
+// the last bits, since its error acts on every step:
+// softplus(d) = max(d, 0) + log(1 + y), y = exp(-|d|).  The exponential's argument
+// is carried in two parts; log(1 + y) = 2 artanh(z), z = y / (2 + y) <= 1/3, by
+// its series up to z^15.
+__device__ __forceinline__ float open_log2(float decay, float rate) {
+    constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) = kLog2e + this
+    const float d = fabsf(decay), x = kLog2e * d;
+    const float rest = fmaf(kLog2e, d, -x) + kLog2eRest * d;
+    float y = exp2_fast(-x);
+    y = fmaf(-kLn2 * rest, y, y);
+    const float w = 2.0f + y;
+    float r = rcp_fast(w);
+    r = fmaf(fmaf(-w, r, 1.0f), r, r);
+    const float z = y * r, t = z * z;
+    float p = 1.0f / 15.0f;
+    p = fmaf(p, t, 1.0f / 13.0f);
+    p = fmaf(p, t, 1.0f / 11.0f);
+    p = fmaf(p, t, 1.0f / 9.0f);
+    p = fmaf(p, t, 1.0f / 7.0f);
+    p = fmaf(p, t, 1.0f / 5.0f);
+    p = fmaf(p, t, 1.0f / 3.0f);
+    p = fmaf(p * t, z, z);
+    const float softplus = fmaf(2.0f, p, fmaxf(decay, 0.0f));
+    return -softplus * (rate * kLog2e);
 }
 
 // -expm1(-w) / w on [0, 0.5]: the polynomial of least largest relative error
@@ -105,11 +119,12 @@ __device__ __forceinline__ float input_scale(float log2a, float a) {
     return __builtin_amdgcn_sqrtf(w < 0.5f ? p * w : fmaf(-a, a, 1.0f));
 }
 
-__device__ __forceinline__ Gates gates(float r, float i, const Rate &c) {
+// k: open_log2 of the channel
+__device__ __forceinline__ Gates gates(float r, float i, float k) {
     Gates g;
     g.open_r = sigmoid_fast(r);
     g.open_i = sigmoid_fast(i);
-    g.log2a = c.k * g.open_r;
+    g.log2a = k * g.open_r;
     g.a = exp2_fast(g.log2a);
     g.s = input_scale(g.log2a, g.a);
     return g;
@@ -122,16 +137,10 @@ __device__ __forceinline__ const T *at(const void *p, int64_t b, int64_t sb, int
     return static_cast<const T *>(p) + b * sb + t * st + c;
 }
 
-// V neighbouring channels of type T
-template <class T, int V>
-struct alignas(sizeof(T) * V) Elements {
-    T v[V];
-};
-
 // Rows are moved by buffer instructions: one descriptor for a tensor's rows of a
-// part, a uniform offset for the row and one register for the lane's, which is
-// past every buffer's end (reads zeros, writes nothing) for a lane past the
-// row's.
+// part, a uniform offset for the row and one register for the lane's channel,
+// which is past every buffer's end (reads zeros, writes nothing) for a lane past
+// the row's.
 using Buffer = __amdgpu_buffer_rsrc_t;
 constexpr int kBufferBytes = 0x7fffffff;
 constexpr uint32_t kNoLane = 0x80000000u;
@@ -141,39 +150,25 @@ __device__ __forceinline__ Buffer buffer_of(const void *p, bool there) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, there ? kBufferBytes : 0, 0x00020000);
 }
 
-// element: the lane's first one, or kNoLane
-template <class T, int V>
-__device__ __forceinline__ Elements<T, V> load_elements(Buffer buffer, uint32_t element, int row) {
-    using E = Elements<T, V>;
-    const int offset = static_cast<int>(element == kNoLane ? kNoLane : element * sizeof(T));
-    if constexpr (sizeof(E) == 2) {
-        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b16(buffer, offset, row, 0));
-    } else if constexpr (sizeof(E) == 4) {
-        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(buffer, offset, row, 0));
-    } else if constexpr (sizeof(E) == 8) {
-        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b64(buffer, offset, row, 0));
+// channel: the lane's, from the buffer's start, or kNoLane; row: in bytes
+template <class T>
+__device__ __forceinline__ T load_channel(Buffer buffer, uint32_t channel, int row) {
+    const int offset = static_cast<int>(channel == kNoLane ? kNoLane : channel * sizeof(T));
+    if constexpr (sizeof(T) == 2) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(buffer, offset, row, 0));
     } else {
-        return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b128(buffer, offset, row, 0));
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(buffer, offset, row, 0));
     }
 }
 
-template <class T, int V>
-__device__ __forceinline__ void store_elements(Buffer buffer, uint32_t element, int row, const float (&f)[V]) {
-    using E = Elements<T, V>;
-    E e;
-#pragma unroll
-    for (int k = 0; k < V; ++k) e.v[k] = static_cast<T>(f[k]);
-    const int offset = static_cast<int>(element == kNoLane ? kNoLane : element * sizeof(T));
-    if constexpr (sizeof(E) == 2) {
-        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, e), buffer, offset, row, 0);
-    } else if constexpr (sizeof(E) == 4) {
-        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, e), buffer, offset, row, 0);
-    } else if constexpr (sizeof(E) == 8) {
-        typedef uint32_t __attribute__((ext_vector_type(2))) Words;
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(Words, e), buffer, offset, row, 0);
+template <class T>
+__device__ __forceinline__ void store_channel(Buffer buffer, uint32_t channel, int row, float f) {
+    const int offset = static_cast<int>(channel == kNoLane ? kNoLane : channel * sizeof(T));
+    const T t = static_cast<T>(f);
+    if constexpr (sizeof(T) == 2) {
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, t), buffer, offset, row, 0);
     } else {
-        typedef uint32_t __attribute__((ext_vector_type(4))) Words;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(Words, e), buffer, offset, row, 0);
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, t), buffer, offset, row, 0);
     }
 }
 
@@ -192,23 +187,6 @@ __device__ __forceinline__ void publish(uint64_t *word, Pair p) {
                        __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// A chunk: its number in the order of the fold, batch item and channels
-struct Place {
-    int64_t chunk, row, b;
-    int c0;            // first channel of the group
-    uint32_t element;  // the lane's first, after it, or kNoLane
-};
-
-// LDS of a workgroup: its parts' pairs, those of earlier chunks, and the state
-// before the chunk
-template <int V>
-struct Shared {
-    Pair parts[kMaxWaves][V][kWave];
-    Pair words[kRound][V][kWave];
-    float heads[V][kWave];
-    uint32_t ticket;
-};
-
 __device__ __forceinline__ uint64_t look(const uint64_t *word) {
     return __hip_atomic_load(word, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
@@ -219,11 +197,26 @@ __device__ __forceinline__ Pair wait_for(const uint64_t *word, uint64_t got) {
     return {__uint_as_float(static_cast<uint32_t>(got)), __uint_as_float(static_cast<uint32_t>(got >> 32))};
 }
 
-// A workgroup's chunk: rows (batch items times channel groups) go by the
-// workgroup's number, and the chunk is the next one of the row in the order of
-// the fold, by a counter (from kPending on) of kCounters that rows share.
-template <int V>
-__device__ __forceinline__ Place place_of(const RecArgs &p, uint64_t *words, int lane, Shared<V> &lds) {
+// LDS of a workgroup: its parts' pairs, those of earlier chunks, and the state
+// before the chunk
+struct Shared {
+    Pair parts[kMaxWaves][kWave];
+    Pair words[kRound][kWave];
+    float heads[kWave];
+    uint32_t ticket;
+};
+
+// A chunk: its number in the order of the fold, row (batch item and 64 channels)
+struct Place {
+    int64_t chunk, row, b;
+    int c0;            // first channel of the row
+    uint32_t channel;  // the lane's, after it, or kNoLane
+};
+
+// A workgroup's chunk: rows go by the workgroup's number, and the chunk is the
+// next one of the row in the order of the fold, by a counter (from kPending on)
+// of kCounters that rows share.
+__device__ __forceinline__ Place place_of(const RecArgs &p, uint64_t *words, int lane, Shared &lds) {
     const uint32_t rows = static_cast<uint32_t>(p.batch) * p.groups;
     const uint32_t lanes = rows < kCounters ? rows : kCounters;
     // (every lane gets as many workgroups as its rows have chunks)
@@ -246,14 +239,13 @@ __device__ __forceinline__ Place place_of(const RecArgs &p, uint64_t *words, int
     at.chunk = chunk;
     at.row = row;
     at.b = b;
-    at.c0 = __builtin_amdgcn_readfirstlane((static_cast<int>(row) - b * p.groups) * kWave * V);
-    at.element = lane * V < static_cast<int>(p.channels) - at.c0 ? lane * V : kNoLane;
+    at.c0 = __builtin_amdgcn_readfirstlane((static_cast<int>(row) - b * p.groups) * kWave);
+    at.channel = lane < static_cast<int>(p.channels) - at.c0 ? lane : kNoLane;
     return at;
 }
 
 // The published pairs of a row: of its chunks, and of kFan chunks each.
-// words: counters, then [chunks][rows][V][64], then [chunks / kFan][rows][V][64]
-template <int V>
+// words: counters, then [chunks][rows][64], then [chunks / kFan][rows][64]
 struct Published {
     uint64_t *pairs, *joined;  // of this row and lane
     int64_t stride;            // to the next chunk's
@@ -261,8 +253,8 @@ struct Published {
     int64_t items, first;      // to fold: in_fan pairs, then the joined ones; of these, in the first round
 
     __device__ __forceinline__ Published(const RecArgs &p, const Place &at, uint64_t *words, int lane) {
-        stride = p.batch * p.groups * (V * kWave);
-        pairs = words + kCounters * kCounterStride + at.row * (V * kWave) + lane;
+        stride = p.batch * p.groups * kWave;
+        pairs = words + kCounters * kCounterStride + at.row * kWave + lane;
         joined = pairs + p.chunks * stride;
         fan = p.chunks > 1 ? at.chunk / kFan : 0;
         in_fan = p.chunks > 1 ? at.chunk % kFan : 0;
@@ -275,80 +267,62 @@ struct Published {
     }
 };
 
-// Each wavefront's first look at a word, together with its inputs: most are there
-template <int V>
+// Each wavefront's first look at its words, together with its inputs: most are there
 struct Early {
-    uint64_t got[kEarly][V];
-    __device__ __forceinline__ void load(const Published<V> &of, int wave, int waves) {
+    uint64_t got[kEarly];
+    __device__ __forceinline__ void load(const Published &of, int wave, int waves) {
 #pragma unroll
         for (int n = 0; n < kEarly; ++n) {
             const int64_t k = wave + n * waves;
-#pragma unroll
-            for (int v = 0; v < V; ++v) got[n][v] = k < of.first ? look(of.item(k) + v * kWave) : kPending;
+            got[n] = k < of.first ? look(of.item(k)) : kPending;
         }
     }
 };
 
-// The state before this chunk into lds.heads, from the one before all (initial)
-// and the pairs of the chunks before it; publishes this chunk's pair, and for
-// the last of kFan chunks that of all of them.  The parts' pairs are in LDS; the
-// wavefronts wait for some words each, and wavefront v (all of them, in turn, if
-// there are fewer) folds channel v of each lane.
-template <int V, bool kBack>
-__device__ __forceinline__ void join_chunks(const RecArgs &p, const Place &at, const Published<V> &of,
-                                            const Early<V> &early, int lane, int wave, int waves,
-                                            const Elements<float, V> &initial, Shared<V> &lds) {
-    Pair own[V], near[V];
-    float h[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (v % waves != wave) continue;
-        h[v] = initial.v[v];
-        near[v] = {1.0f, 0.0f};
-        if (p.chunks == 1) continue;
-        own[v] = lds.parts[kBack ? waves - 1 : 0][v][lane];
-        for (int w = 1; w < waves; ++w) own[v] = own[v].then(lds.parts[kBack ? waves - 1 - w : w][v][lane]);
-        publish(of.pairs + at.chunk * of.stride + v * kWave, own[v]);
+// The state before this chunk, from the one before all (initial) and the pairs
+// of the chunks before it; publishes this chunk's pair, and for the last of kFan
+// chunks that of all of them.  The parts' pairs are in LDS; the wavefronts wait
+// for some words each, and the first one folds them.
+template <bool kBack>
+__device__ __forceinline__ float join_chunks(const RecArgs &p, const Place &at, const Published &of,
+                                             const Early &early, int lane, int wave, int waves, float initial,
+                                             Shared &lds) {
+    if (p.chunks == 1) return initial;
+    Pair own{1.0f, 0.0f}, near{1.0f, 0.0f};
+    float h = initial;
+    if (wave == 0) {
+        for (int w = 0; w < waves; ++w) own = own.then(lds.parts[kBack ? waves - 1 - w : w][lane]);
+        publish(of.pairs + at.chunk * of.stride, own);
     }
     for (int64_t first = 0; first < of.items;) {
         const int64_t left = first == 0 ? of.first : of.items - first;
         const int here = static_cast<int>(left < kRound ? left : kRound);
         for (int k = wave, n = 0; k < here; k += waves, ++n) {
-            const uint64_t *word = of.item(first + k);
+            uint64_t got = kPending;
+            if (first == 0) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                uint64_t got = kPending;
-                if (first == 0) {
-#pragma unroll
-                    for (int m = 0; m < kEarly; ++m) got = n == m ? early.got[m][v] : got;
-                }
-                lds.words[k][v][lane] = wait_for(word + v * kWave, got);
+                for (int m = 0; m < kEarly; ++m) got = n == m ? early.got[m] : got;
             }
+            lds.words[k][lane] = wait_for(of.item(first + k), got);
         }
         __syncthreads();
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (v % waves != wave) continue;
+        if (wave == 0) {
             for (int k = 0; k < here; ++k) {
-                const Pair q = lds.words[k][v][lane];
+                const Pair q = lds.words[k][lane];
                 if (first + k < of.in_fan) {
-                    near[v] = near[v].then(q);
+                    near = near.then(q);
                 } else {
-                    h[v] = q(h[v]);
+                    h = q(h);
                 }
             }
-            if (first == 0 && of.in_fan == kFan - 1) {
-                publish(of.joined + of.fan * of.stride + v * kWave, near[v].then(own[v]));
-            }
+            if (first == 0 && of.in_fan == kFan - 1) publish(of.joined + of.fan * of.stride, near.then(own));
         }
         first += here;
         if (first < of.items) __syncthreads();
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        if (v % waves == wave) lds.heads[v][lane] = near[v](h[v]);
-    }
+    if (wave == 0) lds.heads[lane] = near(h);
     __syncthreads();
+    return lds.heads[lane];
 }
 
 // bits of the resets of steps n0 ..
@@ -387,17 +361,15 @@ __device__ __forceinline__ Rows rows_of(const RecArgs &p, const Place &at, int64
 
 // What a wavefront's part of a chunk needs from memory, requested all at once.
 // (steps past the end stand for the last one; none of an empty part)
-template <class T, int V, bool kReset, int kTensors>
+template <class T, bool kReset, int kTensors>
 struct Part {
-    Elements<T, V> e[kTensors][kSteps];  // r, i, x and, backward, dy
-    Elements<float, V> decay, start, initial;
+    T e[kTensors][kSteps];  // r, i, x and, backward, dy
+    float decay, start, initial;  // (decay: open_log2 of it where that is at hand)
     uint32_t resets;
-    int64_t n0;
     int left;
 
-    __device__ __forceinline__ void load(const RecArgs &p, const Place &at, int64_t n, int lane, const void *gy,
+    __device__ __forceinline__ void load(const RecArgs &p, const Place &at, int64_t n0, int lane, const void *gy,
                                          int64_t sgb, int64_t sgt, const float *starts, const float *first) {
-        n0 = n;
         left = n0 >= p.time ? 0 : p.time - n0 < kSteps ? static_cast<int>(p.time - n0) : kSteps;
         if (left > 0) {
             Rows r = rows_of<T>(p, at, n0, left, p.r, p.srb, p.srt);
@@ -405,224 +377,173 @@ struct Part {
             Rows x = rows_of<T>(p, at, n0, left, p.x, p.sxb, p.sxt);
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) {
-                e[0][s] = load_elements<T, V>(r.buffer, at.element, r.next());
-                e[1][s] = load_elements<T, V>(i.buffer, at.element, i.next());
-                e[2][s] = load_elements<T, V>(x.buffer, at.element, x.next());
+                e[0][s] = load_channel<T>(r.buffer, at.channel, r.next());
+                e[1][s] = load_channel<T>(i.buffer, at.channel, i.next());
+                e[2][s] = load_channel<T>(x.buffer, at.channel, x.next());
             }
             if constexpr (kTensors == 4) {
                 Rows g = rows_of<T>(p, at, n0, left, gy, sgb, sgt);
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) {
-                    e[3][s] = load_elements<T, V>(g.buffer, at.element, g.next());
-                }
+                for (int s = 0; s < kSteps; ++s) e[3][s] = load_channel<T>(g.buffer, at.channel, g.next());
             }
         }
         if constexpr (kTensors == 4) {
             const float *from = starts + (at.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
-            start = load_elements<float, V>(buffer_of(from, left > 0), at.element, 0);
+            start = load_channel<float>(buffer_of(from, left > 0), at.channel, 0);
         }
-        initial = load_elements<float, V>(buffer_of(first + at.b * p.channels + at.c0, first), at.element, 0);
-        decay = load_elements<float, V>(buffer_of(p.decay + at.c0, true), at.element, 0);
+        initial = load_channel<float>(buffer_of(first + at.b * p.channels + at.c0, first), at.channel, 0);
+        decay = load_channel<float>(buffer_of((p.rates ? p.rates : p.decay) + at.c0, true), at.channel, 0);
         resets = reset_bits<kReset>(p, at.b, n0, lane);
     }
 };
 
-template <class T, int V, bool kReset>
-__global__ void __launch_bounds__(kMaxWaves *kWave)
-    recurrence_fwd_kernel(RecArgs p, T *y, float *last, float *starts, uint64_t *words) {
-    __shared__ Shared<V> lds;
-    const int lane = lane_id(), wave = wave_index(), waves = blockDim.x / kWave;
-    const Place here = place_of<V>(p, words, lane, lds);
-    Part<T, V, kReset, 3> part;
-    part.load(p, here, (here.chunk * waves + wave) * kSteps, lane, nullptr, 0, 0, nullptr, p.initial);
-    const Published<V> of(p, here, words, lane);
-    Early<V> early;
-    early.load(of, wave, waves);
-    __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first wait
-    const int left = part.left;
-    const int64_t n0 = part.n0;
-    const uint32_t resets = part.resets;
-    Rate rate[V];
-    float a[kSteps][V], in[kSteps][V], h[V];
-    Pair own[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        rate[v] = channel_rate(part.decay.v[v], p.rate);
-        own[v] = {1.0f, 0.0f};
-    }
-    const auto steps = [&](auto full) {
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const Gates g = gates(static_cast<float>(part.e[0][s].v[v]),
-                                      static_cast<float>(part.e[1][s].v[v]), rate[v]);
-                a[s][v] = there ? g.a : 1.0f;
-                in[s][v] = there ? g.s * g.open_i * static_cast<float>(part.e[2][s].v[v]) : 0.0f;
-                own[v].a = drop ? 0.0f : own[v].a * a[s][v];
-                own[v].b = drop ? in[s][v] : fmaf(a[s][v], own[v].b, in[s][v]);
-            }
-        }
-    };
+// body(true or false as a constant): whether all of the part's steps are there
+template <class Body>
+__device__ __forceinline__ void for_part(int left, Body body) {
     if (left == kSteps) {
-        steps(std::true_type());
+        body(std::true_type());
     } else if (left > 0) {
-        steps(std::false_type());
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) lds.parts[wave][v][lane] = own[v];
-    __syncthreads();
-    join_chunks<V, false>(p, here, of, early, lane, wave, waves, part.initial, lds);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        h[v] = lds.heads[v][lane];
-        for (int w = 0; w < wave; ++w) h[v] = lds.parts[w][v][lane](h[v]);
-    }
-    if (left > 0) {
-        const float *out = starts + (here.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + here.c0;
-        store_elements<float, V>(buffer_of(out, starts), here.element, 0, h);
-        Rows to = rows_of<T>(p, here, n0, left, y, p.time * p.channels, p.channels);
-#pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const bool drop = kReset && (resets >> s & 1);
-#pragma unroll
-            for (int v = 0; v < V; ++v) h[v] = drop ? in[s][v] : fmaf(a[s][v], h[v], in[s][v]);
-            // (a step past the end leaves h and writes the last row again)
-            store_elements<T, V>(to.buffer, here.element, to.next(), h);
-        }
-    }
-    if (last && wave == waves - 1 && here.chunk == p.chunks - 1) {
-        store_elements<float, V>(buffer_of(last + here.b * p.channels + here.c0, true), here.element, 0, h);
+        body(std::false_type());
     }
 }
 
+// Bound by memory and by waiting: 16 x 3751 x 960 bfloat16 takes 128 us, 3.8 TB/s,
+// where the same moves alone take 103.  Five wavefronts a SIMD (96 registers, one
+// spilled) hide more of the waits: 142 us with the four that 97 registers leave.
+template <class T, bool kReset>
+__global__ void __launch_bounds__(kMaxWaves *kWave, 5)
+    recurrence_fwd_kernel(RecArgs p, T *y, float *last, float *starts, uint64_t *words) {
+    __shared__ Shared lds;
+    const int lane = lane_id(), wave = wave_index(), waves = blockDim.x / kWave;
+    const Place at = place_of(p, words, lane, lds);
+    const int64_t n0 = (at.chunk * waves + wave) * kSteps;
+    Part<T, kReset, 3> part;
+    part.load(p, at, n0, lane, nullptr, 0, 0, nullptr, p.initial);
+    const Published of(p, at, words, lane);
+    Early early;
+    early.load(of, wave, waves);
+    __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first wait
+
+    const int left = part.left;
+    const float k = p.rates ? part.decay : open_log2(part.decay, p.rate);
+    float a[kSteps], in[kSteps];
+    Pair own{1.0f, 0.0f};
+    for_part(left, [&](auto full) {
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const bool there = full.value || s < left, drop = kReset && (part.resets >> s & 1);
+            const Gates g = gates(static_cast<float>(part.e[0][s]), static_cast<float>(part.e[1][s]), k);
+            a[s] = there ? g.a : 1.0f;
+            in[s] = there ? g.s * g.open_i * static_cast<float>(part.e[2][s]) : 0.0f;
+            own.a = drop ? 0.0f : own.a * a[s];
+            own.b = drop ? in[s] : fmaf(a[s], own.b, in[s]);
+        }
+    });
+    lds.parts[wave][lane] = own;
+    __syncthreads();
+    float h = join_chunks<false>(p, at, of, early, lane, wave, waves, part.initial, lds);
+    for (int w = 0; w < wave; ++w) h = lds.parts[w][lane](h);
+    if (left > 0) {
+        const float *out = starts + (at.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
+        store_channel<float>(buffer_of(out, starts), at.channel, 0, h);
+        Rows to = rows_of<T>(p, at, n0, left, y, p.time * p.channels, p.channels);
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const bool drop = kReset && (part.resets >> s & 1);
+            h = drop ? in[s] : fmaf(a[s], h, in[s]);
+            // (a step past the end leaves h and writes the last row again)
+            store_channel<T>(to.buffer, at.channel, to.next(), h);
+        }
+    }
+    if (last && wave == waves - 1 && at.chunk == p.chunks - 1) {
+        store_channel<float>(buffer_of(last + at.b * p.channels + at.c0, true), at.channel, 0, h);
+    }
+}
+
+// 16 x 3751 x 960 bfloat16: 209 us, 4.0 TB/s, where the same moves alone take 173
+// and the vector units issue for 136.
+//
 // G as a carry c between steps: g = dy + c, c = a g (0 at a reset), from the
 // last step to the first; chunk 0 of the fold is the last in time.
-template <class T, int V, bool kReset>
+template <class T, bool kReset>
 __global__ void __launch_bounds__(kMaxWaves *kWave)
     recurrence_bwd_kernel(RecArgs p, const T *gy, int64_t sgb, int64_t sgt, const float *g_last,
                           const float *starts, T *gx, T *gr, T *gi, float *decay_part,
                           float *g_initial, uint64_t *words) {
-    __shared__ Shared<V> lds;
-    __shared__ float sums[kMaxWaves][kWave][V];
+    __shared__ Shared lds;
+    __shared__ float sums[kMaxWaves][kWave];
     const int lane = lane_id(), wave = wave_index(), waves = blockDim.x / kWave;
-    const Place here = place_of<V>(p, words, lane, lds);
-    Part<T, V, kReset, 4> part;
-    part.load(p, here, ((p.chunks - 1 - here.chunk) * waves + wave) * kSteps, lane, gy, sgb, sgt, starts, g_last);
-    const Published<V> of(p, here, words, lane);
-    Early<V> early;
+    const Place at = place_of(p, words, lane, lds);
+    const int64_t n0 = ((p.chunks - 1 - at.chunk) * waves + wave) * kSteps;
+    Part<T, kReset, 4> part;
+    part.load(p, at, n0, lane, gy, sgb, sgt, starts, g_last);
+    const Published of(p, at, words, lane);
+    Early early;
     early.load(of, wave, waves);
     __builtin_amdgcn_sched_barrier(0);  // every load is on its way before the first wait
+
     const int left = part.left;
-    const int64_t n0 = part.n0;
-    const uint32_t resets = part.resets;
-    Rate rate[V];
-    float open_r[kSteps][V], a[kSteps][V], g[kSteps][V], c[V], sum[V], h[V];
-    Elements<T, V> ri[kSteps], rx[kSteps];
-    Pair own[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        rate[v] = channel_rate(part.decay.v[v], p.rate);
-        h[v] = part.start.v[v];
-        sum[v] = 0.0f;
-        own[v] = {1.0f, 0.0f};
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        ri[s] = part.e[1][s];
-        rx[s] = part.e[2][s];
-    }
-    const auto towards_start = [&](auto full) {
+    const float k = p.rates ? part.decay : open_log2(part.decay, p.rate);
+    float open_r[kSteps], a[kSteps], g[kSteps];
+    Pair own{1.0f, 0.0f};
+    for_part(left, [&](auto full) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
-            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                open_r[s][v] = sigmoid_fast(static_cast<float>(part.e[0][s].v[v]));
-                a[s][v] = exp2_fast(rate[v].k * open_r[s][v]);
-                g[s][v] = there ? static_cast<float>(part.e[3][s].v[v]) : 0.0f;
-                const float k = there ? a[s][v] : 1.0f;
-                own[v].a = drop ? 0.0f : own[v].a * k;
-                own[v].b = drop ? 0.0f : k * (g[s][v] + own[v].b);
-            }
+            const bool there = full.value || s < left, drop = kReset && (part.resets >> s & 1);
+            open_r[s] = sigmoid_fast(static_cast<float>(part.e[0][s]));
+            a[s] = exp2_fast(k * open_r[s]);
+            g[s] = there ? static_cast<float>(part.e[3][s]) : 0.0f;
+            const float on = there ? a[s] : 1.0f;
+            own.a = drop ? 0.0f : own.a * on;
+            own.b = drop ? 0.0f : on * (g[s] + own.b);
         }
-    };
-    if (left == kSteps) {
-        towards_start(std::true_type());
-    } else if (left > 0) {
-        towards_start(std::false_type());
-    }
-#pragma unroll
-    for (int v = 0; v < V; ++v) lds.parts[wave][v][lane] = own[v];
+    });
+    lds.parts[wave][lane] = own;
     __syncthreads();
-    join_chunks<V, true>(p, here, of, early, lane, wave, waves, part.initial, lds);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        c[v] = lds.heads[v][lane];
-        for (int w = waves - 1; w > wave; --w) c[v] = lds.parts[w][v][lane](c[v]);
-    }
-    const auto gradients = [&](auto full) {
+    float c = join_chunks<true>(p, at, of, early, lane, wave, waves, part.initial, lds), sum = 0.0f;
+    for (int w = waves - 1; w > wave; --w) c = lds.parts[w][lane](c);
+    for_part(left, [&](auto full) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
-            const bool there = full.value || s < left, drop = kReset && (resets >> s & 1);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                g[s][v] += c[v];
-                c[v] = drop ? 0.0f : there ? a[s][v] * g[s][v] : c[v];
-            }
+            const bool there = full.value || s < left, drop = kReset && (part.resets >> s & 1);
+            g[s] += c;
+            c = drop ? 0.0f : there ? a[s] * g[s] : c;
         }
         const int64_t sb = p.time * p.channels;
-        Rows to_x = rows_of<T>(p, here, n0, left, gx, sb, p.channels);
-        Rows to_i = rows_of<T>(p, here, n0, left, gi, sb, p.channels);
-        Rows to_r = rows_of<T>(p, here, n0, left, gr, sb, p.channels);
+        Rows to_x = rows_of<T>(p, at, n0, left, gx, sb, p.channels);
+        Rows to_i = rows_of<T>(p, at, n0, left, gi, sb, p.channels);
+        Rows to_r = rows_of<T>(p, at, n0, left, gr, sb, p.channels);
+        float h = part.start;
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             if (!full.value && s >= left) continue;
-            const bool drop = kReset && (resets >> s & 1);
-            float dx[V], dr[V], di[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float x = static_cast<float>(rx[s].v[v]);
-                const float open_i = sigmoid_fast(static_cast<float>(ri[s].v[v]));
-                const float log2a = rate[v].k * open_r[s][v];
-                const float scale = input_scale(log2a, a[s][v]);
-                const float before = drop ? 0.0f : h[v];
-                const float grad = g[s][v], gate = scale * open_i, kept = a[s][v] * before;
-                const float driven = grad * gate * x;
-                // a^2 / s^2 is infinite where u is 0; times s u (1 - open) it tends to 0
-                const float slope = scale > 0.0f ? a[s][v] * a[s][v] * rcp_fast(scale * scale) : 0.0f;
-                const float du = fmaf(slope, driven, -kept * grad);
-                dx[v] = grad * gate;
-                di[v] = fmaf(-driven, open_i, driven);
-                dr[v] = du * (-kLn2 * log2a) * (1.0f - open_r[s][v]);
-                sum[v] = fmaf(du, open_r[s][v], sum[v]);
-                h[v] = fmaf(gate, x, kept);
-            }
-            store_elements<T, V>(to_x.buffer, here.element, to_x.next(), dx);
-            store_elements<T, V>(to_i.buffer, here.element, to_i.next(), di);
-            store_elements<T, V>(to_r.buffer, here.element, to_r.next(), dr);
+            const float x = static_cast<float>(part.e[2][s]);
+            const float open_i = sigmoid_fast(static_cast<float>(part.e[1][s]));
+            const float log2a = k * open_r[s];
+            const float scale = input_scale(log2a, a[s]);
+            const float before = kReset && (part.resets >> s & 1) ? 0.0f : h;
+            const float gate = scale * open_i, kept = a[s] * before;
+            const float driven = g[s] * gate * x;
+            // a^2 / s^2 is infinite where u is 0; times s u (1 - open) it tends to 0
+            const float slope = scale > 0.0f ? a[s] * a[s] * rcp_fast(scale * scale) : 0.0f;
+            const float du = fmaf(slope, driven, -kept * g[s]);
+            sum = fmaf(du, open_r[s], sum);
+            h = fmaf(gate, x, kept);
+            store_channel<T>(to_x.buffer, at.channel, to_x.next(), g[s] * gate);
+            store_channel<T>(to_i.buffer, at.channel, to_i.next(), fmaf(-driven, open_i, driven));
+            store_channel<T>(to_r.buffer, at.channel, to_r.next(), du * (-kLn2 * log2a) * (1.0f - open_r[s]));
         }
-    };
-    if (left == kSteps) {
-        gradients(std::true_type());
-    } else if (left > 0) {
-        gradients(std::false_type());
-    }
-    if (g_initial && wave == 0 && here.chunk == p.chunks - 1) {
-        store_elements<float, V>(buffer_of(g_initial + here.b * p.channels + here.c0, true), here.element, 0, c);
+    });
+    if (g_initial && wave == 0 && at.chunk == p.chunks - 1) {
+        store_channel<float>(buffer_of(g_initial + at.b * p.channels + at.c0, true), at.channel, 0, c);
     }
     // the chunk's share of ddecay
-#pragma unroll
-    for (int v = 0; v < V; ++v) sums[wave][lane][v] = sum[v];
+    sums[wave][lane] = sum;
     __syncthreads();
     if (wave == 0) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            for (int w = 1; w < waves; ++w) sum[v] += sums[w][lane][v];
-        }
-        float *out = decay_part + (here.chunk * p.batch + here.b) * p.channels + here.c0;
-        store_elements<float, V>(buffer_of(out, true), here.element, 0, sum);
+        for (int w = 1; w < waves; ++w) sum += sums[w][lane];
+        float *out = decay_part + (at.chunk * p.batch + at.b) * p.channels + at.c0;
+        store_channel<float>(buffer_of(out, true), at.channel, 0, sum);
     }
 }
 
@@ -644,13 +565,16 @@ __global__ void __launch_bounds__(kSumRows *kSumChannels)
     __syncthreads();
     if (share != 0 || c >= channels) return;
     for (int k = 1; k < kSumRows; ++k) sum += sums[k][lane];
-    g_decay[c] = sum * channel_rate(decay[c], rate).factor;
+    g_decay[c] = sum * (rate * sigmoid_fast(decay[c]));
 }
 
-__global__ void __launch_bounds__(256) recurrence_fill_kernel(uint64_t *words, int64_t count) {
-    for (int64_t k = int64_t(blockIdx.x) * 256 + threadIdx.x; k < count; k += int64_t(gridDim.x) * 256) {
-        words[k] = kPending;
-    }
+// kPending into all words, and open_log2 of every channel into rates
+__global__ void __launch_bounds__(256)
+    recurrence_fill_kernel(uint64_t *words, int64_t count, const float *decay, int64_t channels, float rate,
+                           float *rates) {
+    const int64_t first = int64_t(blockIdx.x) * 256 + threadIdx.x, step = int64_t(gridDim.x) * 256;
+    for (int64_t c = first; c < channels; c += step) rates[c] = open_log2(decay[c], rate);
+    for (int64_t k = first; k < count; k += step) words[k] = kPending;
 }
 
 template <class T>
@@ -658,7 +582,7 @@ __global__ void __launch_bounds__(kRecThreads) recurrence_step_kernel(RecArgs p,
     const int64_t c = int64_t(blockIdx.x) * kRecThreads + threadIdx.x, b = blockIdx.y;
     if (c >= p.channels) return;
     const Gates g = gates(*at<T>(p.r, b, p.srb, 0, 0, c), *at<T>(p.i, b, p.sib, 0, 0, c),
-                          channel_rate(p.decay[c], p.rate));
+                          open_log2(p.decay[c], p.rate));
     const float x = *at<T>(p.x, b, p.sxb, 0, 0, c);
     const float h = fmaf(g.a, state[b * p.channels + c], g.s * g.open_i * x);
     state[b * p.channels + c] = h;
@@ -702,43 +626,29 @@ static int check_operands(const pesq_recurrence *p) {
     return PESQ_OK;
 }
 
-// How a call is cut up.  V: channels a lane holds, two of a 16 bit type where
-// every pair is aligned.  waves: of a workgroup.
+// How a call is cut up; waves: of a workgroup.
 struct Plan {
-    int v, waves;
-    int64_t chunks, groups, words;
+    int waves;
+    int64_t chunks, groups;
+    int64_t words, bytes;  // of the pairs; of the scratch: these and the channels' rates
 };
 
-static Plan plan_of(const pesq_recurrence *p, bool paired) {
+static Plan plan_of(const pesq_recurrence *p) {
     Plan plan;
-    plan.v = paired ? 2 : 1;
-    plan.groups = cdiv(p->channels, kWave * plan.v);
+    plan.groups = cdiv(p->channels, kWave);
     const int64_t parts = cdiv(p->time, kSteps);
-    // more wavefronts keep the chunks of a long row few: 1 x 64000 x 65 float16 forward
-    // 49 -> 46 us; fewer leave room for two workgroups on a compute unit, one of
-    // which computes while the other waits: 16 x 3751 x 960 bfloat16 201 -> 161 us
+    // Few wavefronts leave room for several workgroups on a compute unit, of which
+    // some compute while others wait (16 x 3751 x 960 bfloat16, forward and backward:
+    // 356 us with 4, 380 us with 8); many keep the chunks of a long row few
+    // (1 x 64000 x 65 float16: 78 us with 16, 103 us with half as many steps each).
     const int most = parts / kWaves > kLongRow ? kMaxWaves : kWaves;
     plan.waves = parts < most ? static_cast<int>(parts < 1 ? 1 : parts) : most;
     plan.chunks = parts < 1 ? 1 : cdiv(parts, plan.waves);
     plan.words = plan.chunks == 1 ? 0
-                                  : kCounters * kCounterStride + (plan.chunks + plan.chunks / kFan) * p->batch *
-                                                                     plan.groups * plan.v * kWave;
+                                  : kCounters * kCounterStride +
+                                        (plan.chunks + plan.chunks / kFan) * p->batch * plan.groups * kWave;
+    plan.bytes = plan.words == 0 ? 0 : (plan.words + cdiv(p->channels, 2)) * int64_t(sizeof(uint64_t));
     return plan;
-}
-
-static bool aligned_pair(const void *p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; }
-
-// whether every 16 bit operand can be taken in pairs of channels
-static bool pairs_fit(const pesq_recurrence *p, const void *g, const int64_t *g_strides,
-                      const void *out0, const void *out1, const void *out2) {
-    if (p->dtype == PESQ_F32 || p->channels % 2) return false;
-    for (int k = 0; k < 6; ++k) {
-        if (p->strides[k / 2][k % 2] % 2) return false;
-    }
-    for (const void *q : {p->x, p->recur_gate, p->input_gate, g, out0, out1, out2}) {
-        if (!aligned_pair(q)) return false;
-    }
-    return !g || (g_strides[0] % 2 == 0 && g_strides[1] % 2 == 0);
 }
 
 static RecArgs kernel_args(const pesq_recurrence *p, const Plan &plan) {
@@ -746,39 +656,36 @@ static RecArgs kernel_args(const pesq_recurrence *p, const Plan &plan) {
             p->strides[0][0], p->strides[0][1], p->strides[1][0], p->strides[1][1],
             p->strides[2][0], p->strides[2][1], p->decay, p->initial, p->reset,
             static_cast<float>(p->rate), p->reverse != 0, plan.chunks,
-            static_cast<int32_t>(plan.groups)};
+            static_cast<int32_t>(plan.groups), nullptr};
 }
 
 static int check_grid(const pesq_recurrence *p, const Plan &plan) {
-    PESQ_CHECK_ARG(plan.chunks * p->batch * plan.groups < (int64_t(1) << 31),
+    PESQ_CHECK_ARG(plan.chunks * p->batch * plan.groups * plan.waves * kWave < (int64_t(1) << 32),
                    "a recurrence of %lld x %lld x %lld is too large", (long long)p->batch,
                    (long long)p->time, (long long)p->channels);
     return PESQ_OK;
 }
 
-// fn(T(), V, reset) with V and reset as constants
+// fn(T(), reset) with reset as a constant
 template <class Fn>
-static void with_variant(const pesq_recurrence *p, const Plan &plan, Fn fn) {
-    const auto with_reset = [&](auto type, auto v) {
-        if (p->reset) {
-            fn(type, v, std::true_type());
-        } else {
-            fn(type, v, std::false_type());
-        }
-    };
+static void with_variant(const pesq_recurrence *p, Fn fn) {
     with_type(p->dtype, [&](auto type) {
-        if constexpr (sizeof(type) == 2) {
-            if (plan.v == 2) return with_reset(type, std::integral_constant<int, 2>());
+        if (p->reset) {
+            fn(type, std::true_type());
+        } else {
+            fn(type, std::false_type());
         }
-        with_reset(type, std::integral_constant<int, 1>());
     });
 }
 
-static void fill_words(const Plan &plan, uint64_t *words, hipStream_t stream) {
+// Makes the scratch of a call of several chunks a row ready, and the rates known to it
+static void fill_words(RecArgs &args, const Plan &plan, uint64_t *words, hipStream_t stream) {
     if (plan.words == 0) return;
+    float *rates = reinterpret_cast<float *>(words + plan.words);
     const int64_t blocks = cdiv(plan.words, 1024);
     recurrence_fill_kernel<<<static_cast<unsigned>(blocks < 2048 ? blocks : 2048), 256, 0, stream>>>(
-        words, plan.words);
+        words, plan.words, args.decay, args.channels, args.rate, rates);
+    args.rates = rates;
 }
 
 static unsigned grid_of(const pesq_recurrence *p, const Plan &plan) {
@@ -793,10 +700,10 @@ extern "C" int pesq_recurrence_workspace(const pesq_recurrence *p, size_t *start
                                          size_t *backward) {
     if (int st = check_recurrence(p)) return st;
     const size_t states = size_t(p->batch) * p->channels * sizeof(float);
-    const Plan plan = plan_of(p, true);  // single channels need no more
+    const Plan plan = plan_of(p);
     if (starts) *starts = states * cdiv(p->time, kSteps);
-    if (forward) *forward = plan.words * sizeof(uint64_t);
-    if (backward) *backward = plan.words * sizeof(uint64_t) + states * plan.chunks;
+    if (forward) *forward = plan.bytes;
+    if (backward) *backward = plan.bytes + states * plan.chunks;
     return PESQ_OK;
 }
 
@@ -805,16 +712,17 @@ extern "C" int pesq_recurrence_forward(const pesq_recurrence *p, void *y, float 
     if (int st = check_operands(p)) return st;
     if (empty(p)) return PESQ_OK;
     PESQ_CHECK_ARG(y || p->time == 0, "null argument");
-    const Plan plan = plan_of(p, pairs_fit(p, nullptr, nullptr, y, nullptr, nullptr));
+    const Plan plan = plan_of(p);
     if (int st = check_grid(p, plan)) return st;
     PESQ_CHECK_ARG(workspace || plan.words == 0, "null argument");
     uint64_t *words = static_cast<uint64_t *>(workspace);
-    fill_words(plan, words, stream);
-    with_variant(p, plan, [&](auto type, auto v, auto reset) {
+    RecArgs args = kernel_args(p, plan);
+    fill_words(args, plan, words, stream);
+    with_variant(p, [&](auto type, auto reset) {
         using T = decltype(type);
-        recurrence_fwd_kernel<T, v.value, reset.value>
+        recurrence_fwd_kernel<T, reset.value>
             <<<grid_of(p, plan), plan.waves * kWave, 0, stream>>>(
-                kernel_args(p, plan), static_cast<T *>(y), last, starts, words);
+                args, static_cast<T *>(y), last, starts, words);
     });
     PESQ_CHECK_LAUNCH("pesq_recurrence_forward");
     return PESQ_OK;
@@ -831,17 +739,18 @@ extern "C" int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_
     if (p->channels == 0) return PESQ_OK;
     PESQ_CHECK_ARG(empty(p) || (workspace && (starts || p->time == 0)), "null argument");
     PESQ_CHECK_ARG(!g_decay || p->decay, "null argument");
-    const Plan plan = plan_of(p, pairs_fit(p, g_y, g_strides, g_x, g_recur, g_input));
+    const Plan plan = plan_of(p);
     if (int st = check_grid(p, plan)) return st;
     uint64_t *words = static_cast<uint64_t *>(workspace);
-    float *part = reinterpret_cast<float *>(words + plan.words);
+    float *part = reinterpret_cast<float *>(static_cast<char *>(workspace) + plan.bytes);
     if (p->batch > 0) {
-        fill_words(plan, words, stream);
-        with_variant(p, plan, [&](auto type, auto v, auto reset) {
+        RecArgs args = kernel_args(p, plan);
+        fill_words(args, plan, words, stream);
+        with_variant(p, [&](auto type, auto reset) {
             using T = decltype(type);
-            recurrence_bwd_kernel<T, v.value, reset.value>
+            recurrence_bwd_kernel<T, reset.value>
                 <<<grid_of(p, plan), plan.waves * kWave, 0, stream>>>(
-                    kernel_args(p, plan), static_cast<const T *>(g_y), g_y ? g_strides[0] : 0,
+                    args, static_cast<const T *>(g_y), g_y ? g_strides[0] : 0,
                     g_y ? g_strides[1] : 0, g_last, starts, static_cast<T *>(g_x),
                     static_cast<T *>(g_recur), static_cast<T *>(g_input), part, g_initial, words);
         });
