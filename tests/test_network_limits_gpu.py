@@ -1,0 +1,166 @@
+"""The network operators beyond 32 bit offsets, in HIP graphs and on streams at once.
+
+Each result is compared with the same call on small, contiguous, eager tensors,
+bit for bit: neither strides nor how the call is made may change it.
+"""
+
+import pytest
+import torch
+
+from torch_pesq.hip_ops.adamw import HipAdamW
+from torch_pesq.hip_ops.norm import residual_norm
+from torch_pesq.hip_ops.recurrence import gated_recurrence
+
+pytestmark = pytest.mark.gpu
+
+FAR = 2**31 + 2**20  # elements
+
+
+def _recurrence_inputs(shape, dtype=torch.bfloat16, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    t = [torch.randn(shape, generator=g, device="cuda").to(dtype) for _ in range(3)]
+    decay = -4.0 - 4.0 * torch.rand(shape[-1], generator=g, device="cuda")
+    up = torch.randn(shape, generator=g, device="cuda").to(dtype)
+    return t, decay, up
+
+
+def _recurrence_step(t, decay, up):
+    leaves = [v.detach().requires_grad_() for v in t]
+    y, last = gated_recurrence(*leaves, decay)
+    return [y.detach(), last.detach(), *torch.autograd.grad(y, leaves, up)]
+
+
+def _same(got, want):
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_recurrence_rows_far_apart():
+    t, decay, up = _recurrence_inputs((3, 300, 70))
+    want = _recurrence_step(t, decay, up)
+    far = torch.zeros(2 * FAR + 10**6, dtype=torch.bfloat16, device="cuda")
+    spread = far.as_strided(t[0].shape, (FAR, 70, 1))
+    spread.copy_(t[0])
+    _same(_recurrence_step([spread, t[1], t[2]], decay, up), want)
+    up_far = far.as_strided(up.shape, (FAR, 80, 1), 500_000)
+    up_far.copy_(up)
+    _same(_recurrence_step([t[0], t[1], t[2]], decay, up_far), want)
+    # steps as far apart as the operator takes them, and further: copied
+    for stride in (2**26 - 2, 2**26 + 2):
+        steps = far.as_strided((1, 60, 70), (0, stride, 1))
+        part = [v[:1, :60].contiguous() for v in t]
+        steps.copy_(part[1])
+        _same(_recurrence_step([part[0], steps, part[2]], decay, up[:1, :60].contiguous()),
+              _recurrence_step(part, decay, up[:1, :60].contiguous()))
+
+
+def test_recurrence_larger_than_32_bits():
+    """More than 2^31 elements of y: the last rows against the same rows alone."""
+
+    shape = (34, 64000, 1024)
+    x = torch.full((1, 1, 1), 0.5, dtype=torch.bfloat16, device="cuda").expand(shape)
+    tail, decay, _ = _recurrence_inputs((1, 64000, 1024), seed=3)
+    gate = tail[1].expand(shape)
+    y, last = gated_recurrence(x, gate, gate, decay)
+    want, want_last = gated_recurrence(x[:1], tail[1], tail[1], decay)
+    for row in (0, 32, 33):
+        assert torch.equal(y[row], want[0]) and torch.equal(last[row], want_last[0])
+
+
+def test_norm_rows_far_apart():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x, branch, gate = (torch.randn(5, 264, generator=g, device="cuda").bfloat16() for _ in range(3))
+    w = torch.rand(264, generator=g, device="cuda") + 0.5
+
+    def step(x, branch, gate):
+        leaves = [v.detach().requires_grad_() for v in (x, branch, gate)]
+        out = residual_norm(leaves[0], leaves[1], w, gate=leaves[2], scale=w, next_weight=w)
+        return [*(o.detach() for o in out), *torch.autograd.grad(out, leaves, (branch, gate))]
+
+    far = torch.zeros(3 * (FAR // 2) + 4 * FAR // 4, dtype=torch.bfloat16, device="cuda")
+    spread = far.as_strided(x.shape, (FAR // 2, 1))
+    spread.copy_(branch)
+    _same(step(x, spread, gate), step(x, branch, gate))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_tensor_of_more_than_2_31_elements(bits):
+    count = 2**31 + 777
+    p = torch.nn.Parameter(torch.full((count,), 0.5, dtype=torch.bfloat16, device="cuda"))
+    p.grad = torch.zeros(count, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(6)
+    end = torch.randn(3000, generator=g, device="cuda").bfloat16()
+    p.grad[-3000:] = end
+    small = torch.nn.Parameter(torch.full((3000,), 0.5, dtype=torch.bfloat16, device="cuda"))
+    small.grad = end.clone()
+    for q in (p, small):
+        HipAdamW([q], lr=1e-1, state_bits=bits).step()
+    assert torch.equal(p.detach()[-3000:], small.detach())
+    assert (p.detach()[:-3000] == p.detach()[0]).all()
+
+
+def test_forward_in_a_graph():
+    """Captured once, replayed with new inputs between eager calls."""
+
+    shape = (3, 700, 96)
+    t, decay, _ = _recurrence_inputs(shape, seed=7)
+    w = torch.rand(96, device="cuda") + 0.5
+
+    def call():
+        y, last = gated_recurrence(*t, decay)
+        x, n = residual_norm(t[0], y, w, gate=t[1], next_weight=w)
+        return [y, last, x, n]
+
+    with torch.no_grad():
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        for seed in range(8, 13):
+            fresh, _, _ = _recurrence_inputs(shape, seed=seed)
+            for v, f in zip(t, fresh):
+                v.copy_(f)
+            graph.replay()
+            torch.cuda.synchronize()
+            _same(out, call())
+
+
+def test_optimizer_step_in_a_graph():
+    """A captured step repeats its own step's corrections: the same as an eager one
+    from the same count."""
+
+    for bits in (32, 8):
+        p, q = (torch.nn.Parameter(torch.linspace(-1, 1, 5000, device="cuda")) for _ in range(2))
+        p.grad, q.grad = (torch.linspace(1, -1, 5000, device="cuda") for _ in range(2))
+        captured, eager = HipAdamW([p], state_bits=bits), HipAdamW([q], state_bits=bits)
+        captured.moments()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            captured.step()
+        graph.replay()
+        eager.step()
+        torch.cuda.synchronize()
+        assert torch.equal(p, q)
+        _same(captured.moments(), eager.moments())
+
+
+def test_streams_at_once():
+    """Two streams' recurrences of many chunks at the same time: each waits for its
+    own pairs only."""
+
+    cases = [_recurrence_inputs((2, 9000, 130), seed=20), _recurrence_inputs((40, 1500, 96), seed=21)]
+    want = [_recurrence_step(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(5):
+        for k, (c, s) in enumerate(zip(cases, streams)):
+            with torch.cuda.stream(s):
+                got[k] = _recurrence_step(*c)
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        _same(a, b)
