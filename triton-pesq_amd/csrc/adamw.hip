@@ -89,9 +89,8 @@ __device__ __forceinline__ void values(uint32_t cm, uint32_t cv, float sm, float
     }
 }
 
-template <class T>
-struct alignas(sizeof(T) * kLane) Lane {
-    T v[kLane];
+struct alignas(16) Lane {
+    float v[kLane];
 };
 
 // Codes are those of correctly rounded roots.  The hardware's root (one unit in
@@ -168,9 +167,9 @@ __device__ __forceinline__ float inverse_of(float scale) { return scale == 0.0f 
 
 // a lane's neighbours from element `at` of a tensor; zeros past its end
 template <class T>
-__device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count, bool aligned, float (&out)[kLane]) {
-    if (aligned && at + kLane <= count) {
-        const Lane<T> e = *reinterpret_cast<const Lane<T> *>(p + at);
+__device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count, float (&out)[kLane]) {
+    if (at + kLane <= count) {
+        const auto e = load_neighbours<T, kLane>(p + at);
 #pragma unroll
         for (int k = 0; k < kLane; ++k) out[k] = static_cast<float>(e.v[k]);
     } else {
@@ -180,12 +179,12 @@ __device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count,
 }
 
 template <class T>
-__device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, bool aligned, const float (&f)[kLane]) {
-    if (aligned && at + kLane <= count) {
-        Lane<T> e;
+__device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, const float (&f)[kLane]) {
+    if (at + kLane <= count) {
+        Neighbours<T, kLane> e;
 #pragma unroll
         for (int k = 0; k < kLane; ++k) e.v[k] = static_cast<T>(f[k]);
-        *reinterpret_cast<Lane<T> *>(p + at) = e;
+        store_neighbours<T, kLane>(p + at, e);
     } else {
 #pragma unroll
         for (int k = 0; k < kLane; ++k) {
@@ -214,8 +213,6 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     const int64_t count = t.count, block0 = int64_t(tile) * kTileBlocks + wave_index() * kMine;
     T *param = static_cast<T *>(t.param);
     const T *grad = static_cast<const T *>(t.grad);
-    const bool aligned =
-        (reinterpret_cast<uintptr_t>(param) | reinterpret_cast<uintptr_t>(grad)) % sizeof(Lane<T>) == 0;
     const AdamArgs a = list.args;
 
     float p[kMine][kLane], g[kMine][kLane], m[kMine][kLane], v[kMine][kLane];
@@ -223,16 +220,16 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     for (int n = 0; n < kMine; ++n) {
         const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
         if (block * kBlock >= count) break;
-        load_lane(param, at, count, aligned, p[n]);
-        load_lane(grad, at, count, aligned, g[n]);
+        load_lane(param, at, count, p[n]);
+        load_lane(grad, at, count, g[n]);
         const int64_t held = int64_t(t.block) + block;
         if constexpr (kEight) {
             values(static_cast<const uint32_t *>(list.m)[held * kWave + lane],
                    static_cast<const uint32_t *>(list.v)[held * kWave + lane], list.m_scale[held],
                    list.v_scale[held], m[n], v[n]);
         } else {
-            const Lane<float> em = static_cast<const Lane<float> *>(list.m)[held * kWave + lane];
-            const Lane<float> ev = static_cast<const Lane<float> *>(list.v)[held * kWave + lane];
+            const Lane em = static_cast<const Lane *>(list.m)[held * kWave + lane];
+            const Lane ev = static_cast<const Lane *>(list.v)[held * kWave + lane];
 #pragma unroll
             for (int k = 0; k < kLane; ++k) {
                 m[n][k] = em.v[k];
@@ -247,7 +244,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
         // (past the end m, v and g are 0, and the moments stay 0)
 #pragma unroll
         for (int k = 0; k < kLane; ++k) p[n][k] = adamw(p[n][k], g[n][k], m[n][k], v[n][k], a);
-        store_lane(param, at, count, aligned, p[n]);
+        store_lane(param, at, count, p[n]);
         const int64_t held = int64_t(t.block) + block;
         if constexpr (kEight) {
             const float sm = block_scale(m[n]), sv = block_scale(v[n]);
@@ -261,14 +258,14 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
                 list.v_scale[held] = sv;
             }
         } else {
-            Lane<float> em, ev;
+            Lane em, ev;
 #pragma unroll
             for (int k = 0; k < kLane; ++k) {
                 em.v[k] = m[n][k];
                 ev.v[k] = v[n][k];
             }
-            static_cast<Lane<float> *>(list.m)[held * kWave + lane] = em;
-            static_cast<Lane<float> *>(list.v)[held * kWave + lane] = ev;
+            static_cast<Lane *>(list.m)[held * kWave + lane] = em;
+            static_cast<Lane *>(list.v)[held * kWave + lane] = ev;
         }
     }
 }
@@ -279,10 +276,10 @@ __global__ void __launch_bounds__(kAdamThreads)
     const int64_t block = int64_t(blockIdx.x) * (kAdamThreads / kWave) + wave_index();
     if (block >= blocks) return;
     const int64_t at = block * kWave + lane_id();
-    Lane<float> em, ev;
+    Lane em, ev;
     values(m[at], v[at], m_scale[block], v_scale[block], em.v, ev.v);
-    reinterpret_cast<Lane<float> *>(m_out)[at] = em;
-    reinterpret_cast<Lane<float> *>(v_out)[at] = ev;
+    reinterpret_cast<Lane *>(m_out)[at] = em;
+    reinterpret_cast<Lane *>(v_out)[at] = ev;
 }
 
 // the launch of a list of `tiles` tiles

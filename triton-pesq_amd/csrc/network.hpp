@@ -39,4 +39,36 @@ __device__ __forceinline__ float sigmoid_fast(float x) {
     return rcp_fast(1.0f + exp2_fast(-kLog2e * x));
 }
 
+// V neighbouring elements moved at once from and to any element of a tensor:
+// the hardware takes 16 byte accesses at any address, so rows of odd lengths
+// need no element by element variant, only their ends do.
+template <class T, int V>
+struct Neighbours {
+    T v[V];
+};
+
+template <class T, int V>
+__device__ __forceinline__ Neighbours<T, V> load_neighbours(const T *p) {
+    constexpr int kBytes = sizeof(T) * V, kMove = kBytes < 16 ? kBytes : 16;
+    typedef uint32_t __attribute__((ext_vector_type(kMove / 4), aligned(sizeof(T)))) Move;
+    struct Moves {
+        Move m[kBytes / kMove];
+    } moves;
+#pragma unroll
+    for (int k = 0; k < kBytes / kMove; ++k) moves.m[k] = reinterpret_cast<const Move *>(p)[k];
+    return __builtin_bit_cast(Neighbours<T, V>, moves);
+}
+
+template <class T, int V>
+__device__ __forceinline__ void store_neighbours(T *p, const Neighbours<T, V> &e) {
+    constexpr int kBytes = sizeof(T) * V, kMove = kBytes < 16 ? kBytes : 16;
+    typedef uint32_t __attribute__((ext_vector_type(kMove / 4), aligned(sizeof(T)))) Move;
+    struct Moves {
+        Move m[kBytes / kMove];
+    };
+    const Moves moves = __builtin_bit_cast(Moves, e);
+#pragma unroll
+    for (int k = 0; k < kBytes / kMove; ++k) reinterpret_cast<Move *>(p)[k] = moves.m[k];
+}
+
 }  // namespace pesq

@@ -41,11 +41,7 @@ struct NormArgs {
     const float *post, *scale, *next;
     float eps;
     int lanes;  // per row
-};
-
-template <class T, int V>
-struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Vec {
-    T v[V];
+    int whole;  // channels in whole vectors
 };
 
 template <int kCtrl>
@@ -97,144 +93,170 @@ struct NormPlace {
         : lane(threadIdx.x % lanes), group(threadIdx.x / lanes), groups(blockDim.x / lanes) {}
 };
 
-// E elements of a row by this thread: vectors of V neighbours, lanes V apart
-template <int V, int E, class T>
-__device__ __forceinline__ void load_row(const T *row, const NormArgs &p, int lane, float (&out)[E]) {
+// N elements of a row by this thread: E in vectors of V neighbours, lanes V
+// apart, and, where the row does not end with a vector (N = E + 1), one of the
+// few left.  Zeros past the end.
+template <int V, int E, int N, class T>
+__device__ __forceinline__ void load_row(const T *row, const NormArgs &p, int lane, float (&out)[N]) {
 #pragma unroll
     for (int j = 0; j < E / V; ++j) {
         const int c = (j * p.lanes + lane) * V;
-        Vec<T, V> e{};
-        if (c < p.channels) e = *reinterpret_cast<const Vec<T, V> *>(row + c);
+        Neighbours<T, V> e{};
+        if (c < p.whole) e = load_neighbours<T, V>(row + c);
 #pragma unroll
         for (int k = 0; k < V; ++k) out[j * V + k] = static_cast<float>(e.v[k]);
     }
+    if constexpr (N > E) {
+        T t{};
+        if (p.whole + lane < p.channels) t = row[p.whole + lane];
+        out[E] = static_cast<float>(t);
+    }
 }
 
-template <int V, int E, class T>
-__device__ __forceinline__ void store_row(T *row, const NormArgs &p, int lane, const float (&f)[E]) {
+template <int V, int E, int N, class T>
+__device__ __forceinline__ void store_row(T *row, const NormArgs &p, int lane, const float (&f)[N]) {
 #pragma unroll
     for (int j = 0; j < E / V; ++j) {
         const int c = (j * p.lanes + lane) * V;
-        Vec<T, V> e;
+        Neighbours<T, V> e;
 #pragma unroll
         for (int k = 0; k < V; ++k) e.v[k] = static_cast<T>(f[j * V + k]);
-        if (c < p.channels) *reinterpret_cast<Vec<T, V> *>(row + c) = e;
+        if (c < p.whole) store_neighbours<T, V>(row + c, e);
+    }
+    if constexpr (N > E) {
+        if (p.whole + lane < p.channels) row[p.whole + lane] = static_cast<T>(f[E]);
     }
 }
 
 // a weight by this thread, `otherwise` where there is none
-template <int V, int E>
+template <int V, int E, int N>
 __device__ __forceinline__ void load_weight(const float *w, const NormArgs &p, int lane, float otherwise,
-                                            float (&out)[E]) {
+                                            float (&out)[N]) {
+    if (w) return load_row<V, E>(w, p, lane, out);
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = otherwise;
+}
+
+// use(channel, element) for each of a thread's elements, by vectors and alone
+template <int V, int E, int N, class Use>
+__device__ __forceinline__ void each_channel(const NormArgs &p, int lane, Use use) {
 #pragma unroll
     for (int j = 0; j < E / V; ++j) {
         const int c = (j * p.lanes + lane) * V;
+        if (c < p.whole) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) out[j * V + k] = c >= p.channels ? 0.0f : w ? w[c + k] : otherwise;
+            for (int k = 0; k < V; ++k) use(c + k, j * V + k);
+        }
+    }
+    if constexpr (N > E) {
+        if (p.whole + lane < p.channels) use(p.whole + lane, E);
     }
 }
 
-// V: elements of a 16 byte move of T, or 1 where rows are not aligned; E: of a thread
-template <class S, class T, int V, int E, int kWidth>
+// V: elements of a 16 byte move of T; E: of a thread in such; kTail: whether rows
+// end with part of one
+template <class S, class T, int V, int E, int kWidth, bool kTail>
 __global__ void __launch_bounds__(kMostNormThreads)
     residual_norm_fwd_kernel(NormArgs p, S *x_out, T *n_out, float *inv) {
     __shared__ float buffers[2][kMostNormThreads / kWave];
+    constexpr int N = E + kTail;
     const NormPlace at(p.lanes);
     RowSum<kWidth> row_sum{buffers, p.lanes / kWave, static_cast<int>(threadIdx.x) / p.lanes * (p.lanes / kWave)};
     const float share = 1.0f / static_cast<float>(p.channels);
-    float both[E], next[E];
+    float both[N], next[N];
     if (p.branch) {
-        load_weight<V>(p.post, p, at.lane, 1.0f, both);
-        load_weight<V>(p.scale, p, at.lane, 1.0f, next);
+        load_weight<V, E>(p.post, p, at.lane, 1.0f, both);
+        load_weight<V, E>(p.scale, p, at.lane, 1.0f, next);
 #pragma unroll
-        for (int k = 0; k < E; ++k) both[k] *= next[k];
+        for (int k = 0; k < N; ++k) both[k] *= next[k];
     }
-    load_weight<V>(p.next, p, at.lane, 1.0f, next);
+    load_weight<V, E>(p.next, p, at.lane, 1.0f, next);
     const int64_t step = int64_t(gridDim.x) * at.groups;
     for (int64_t first = int64_t(blockIdx.x) * at.groups; first < p.rows; first += step) {
         // (every lane takes part in the sums)
         const bool there = first + at.group < p.rows;
         const int64_t row = there ? first + at.group : p.rows - 1;
-        float x[E], y[E];
-        load_row<V>(static_cast<const S *>(p.x) + row * p.sx, p, at.lane, x);
+        float x[N], y[N];
+        load_row<V, E>(static_cast<const S *>(p.x) + row * p.sx, p, at.lane, x);
         if (p.branch) {
-            load_row<V>(static_cast<const T *>(p.branch) + row * p.sb, p, at.lane, y);
+            load_row<V, E>(static_cast<const T *>(p.branch) + row * p.sb, p, at.lane, y);
             if (p.gate) {
-                float g[E];
-                load_row<V>(static_cast<const T *>(p.gate) + row * p.sg, p, at.lane, g);
+                float g[N];
+                load_row<V, E>(static_cast<const T *>(p.gate) + row * p.sg, p, at.lane, g);
 #pragma unroll
-                for (int k = 0; k < E; ++k) y[k] *= g[k] * sigmoid_fast(g[k]);
+                for (int k = 0; k < N; ++k) y[k] *= g[k] * sigmoid_fast(g[k]);
             }
             float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < E; ++k) sum = fmaf(y[k], y[k], sum);
+            for (int k = 0; k < N; ++k) sum = fmaf(y[k], y[k], sum);
             const float inv_y = 1.0f / sqrtf(fmaf(row_sum(sum), share, p.eps));
             if (inv && there && at.lane == 0) inv[2 * row] = inv_y;
 #pragma unroll
-            for (int k = 0; k < E; ++k) x[k] = fmaf(both[k], y[k] * inv_y, x[k]);
-            if (there) store_row<V>(x_out + row * p.channels, p, at.lane, x);
+            for (int k = 0; k < N; ++k) x[k] = fmaf(both[k], y[k] * inv_y, x[k]);
+            if (there) store_row<V, E>(x_out + row * p.channels, p, at.lane, x);
         }
         if (p.next) {
             float sum = 0.0f;
 #pragma unroll
-            for (int k = 0; k < E; ++k) sum = fmaf(x[k], x[k], sum);
+            for (int k = 0; k < N; ++k) sum = fmaf(x[k], x[k], sum);
             const float inv_x = 1.0f / sqrtf(fmaf(row_sum(sum), share, p.eps));
             if (inv && there && at.lane == 0) inv[2 * row + 1] = inv_x;
 #pragma unroll
-            for (int k = 0; k < E; ++k) x[k] *= inv_x * next[k];
-            if (there) store_row<V>(n_out + row * p.channels, p, at.lane, x);
+            for (int k = 0; k < N; ++k) x[k] *= inv_x * next[k];
+            if (there) store_row<V, E>(n_out + row * p.channels, p, at.lane, x);
         }
     }
 }
 
 // part[workgroup][2][channels]: the workgroup's sums of gx y^ and dn x'^
-template <class S, class T, int V, int E, int kWidth>
+template <class S, class T, int V, int E, int kWidth, bool kTail>
 __global__ void __launch_bounds__(kMostNormThreads)
     residual_norm_bwd_kernel(NormArgs p, const S *g_out, int64_t sgo, const T *g_next, int64_t sgn,
                              const float *inv, S *g_x, T *g_branch, T *g_gate, float *part) {
     __shared__ float buffers[2][kMostNormThreads / kWave];
-    __shared__ float sums[2 * E * kNormThreads / 2];  // (several groups: half the threads each at most)
+    __shared__ float sums[2 * (E * kNormThreads / 2 + V)];  // (several groups: half the threads each at most)
+    constexpr int N = E + kTail;
     const NormPlace at(p.lanes);
     RowSum<kWidth> row_sum{buffers, p.lanes / kWave, static_cast<int>(threadIdx.x) / p.lanes * (p.lanes / kWave)};
     const float share = 1.0f / static_cast<float>(p.channels);
-    float both[E], next[E], sum_both[E], sum_next[E];
-    load_weight<V>(p.post, p, at.lane, 1.0f, both);
-    load_weight<V>(p.scale, p, at.lane, 1.0f, next);
+    float both[N], next[N], sum_both[N], sum_next[N];
+    load_weight<V, E>(p.post, p, at.lane, 1.0f, both);
+    load_weight<V, E>(p.scale, p, at.lane, 1.0f, next);
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
+    for (int k = 0; k < N; ++k) {
         both[k] *= next[k];
         sum_both[k] = sum_next[k] = 0.0f;
     }
-    load_weight<V>(p.next, p, at.lane, 1.0f, next);
+    load_weight<V, E>(p.next, p, at.lane, 1.0f, next);
     const int64_t step = int64_t(gridDim.x) * at.groups;
     for (int64_t first = int64_t(blockIdx.x) * at.groups; first < p.rows; first += step) {
         const bool there = first + at.group < p.rows;
         const int64_t row = there ? first + at.group : p.rows - 1;
-        float x[E], b[E], a[E], gx[E];
-        load_row<V>(static_cast<const S *>(p.x) + row * p.sx, p, at.lane, x);
-        if (p.branch) load_row<V>(static_cast<const T *>(p.branch) + row * p.sb, p, at.lane, b);
-        if (p.gate) load_row<V>(static_cast<const T *>(p.gate) + row * p.sg, p, at.lane, a);
+        float x[N], b[N], a[N], gx[N];
+        load_row<V, E>(static_cast<const S *>(p.x) + row * p.sx, p, at.lane, x);
+        if (p.branch) load_row<V, E>(static_cast<const T *>(p.branch) + row * p.sb, p, at.lane, b);
+        if (p.gate) load_row<V, E>(static_cast<const T *>(p.gate) + row * p.sg, p, at.lane, a);
         if (g_out) {
-            load_row<V>(g_out + row * sgo, p, at.lane, gx);
+            load_row<V, E>(g_out + row * sgo, p, at.lane, gx);
         } else {
 #pragma unroll
-            for (int k = 0; k < E; ++k) gx[k] = 0.0f;
+            for (int k = 0; k < N; ++k) gx[k] = 0.0f;
         }
         const float inv_y = inv[2 * row], inv_x = inv[2 * row + 1];
-        float unit[E];  // y^
+        float unit[N];  // y^
         if (p.branch) {
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
+            for (int k = 0; k < N; ++k) {
                 unit[k] = b[k] * inv_y;
                 if (p.gate) unit[k] *= a[k] * sigmoid_fast(a[k]);
                 x[k] = fmaf(both[k], unit[k], x[k]);
             }
         }
         if (g_next) {
-            float v[E], sum = 0.0f;
-            load_row<V>(g_next + row * sgn, p, at.lane, v);
+            float v[N], sum = 0.0f;
+            load_row<V, E>(g_next + row * sgn, p, at.lane, v);
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
+            for (int k = 0; k < N; ++k) {
                 x[k] *= inv_x;  // x'^
                 if (there) sum_next[k] = fmaf(v[k], x[k], sum_next[k]);
                 v[k] *= next[k];
@@ -242,56 +264,50 @@ __global__ void __launch_bounds__(kMostNormThreads)
             }
             const float mean = row_sum(sum) * share;
 #pragma unroll
-            for (int k = 0; k < E; ++k) gx[k] = fmaf(inv_x, fmaf(-x[k], mean, v[k]), gx[k]);
+            for (int k = 0; k < N; ++k) gx[k] = fmaf(inv_x, fmaf(-x[k], mean, v[k]), gx[k]);
         }
-        if (g_x && there) store_row<V>(g_x + row * p.channels, p, at.lane, gx);
+        if (g_x && there) store_row<V, E>(g_x + row * p.channels, p, at.lane, gx);
         if (!p.branch) continue;
         float sum = 0.0f;
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
+        for (int k = 0; k < N; ++k) {
             if (there) sum_both[k] = fmaf(gx[k], unit[k], sum_both[k]);
             gx[k] *= both[k];
             sum = fmaf(gx[k], unit[k], sum);
         }
         const float mean = row_sum(sum) * share;
 #pragma unroll
-        for (int k = 0; k < E; ++k) gx[k] = inv_y * fmaf(-unit[k], mean, gx[k]);  // gy
+        for (int k = 0; k < N; ++k) gx[k] = inv_y * fmaf(-unit[k], mean, gx[k]);  // gy
         if (p.gate) {
-            float dgate[E];
+            float dgate[N];
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
+            for (int k = 0; k < N; ++k) {
                 const float sig = sigmoid_fast(a[k]);
                 dgate[k] = gx[k] * b[k] * sig * fmaf(a[k], 1.0f - sig, 1.0f);
                 gx[k] *= a[k] * sig;
             }
-            if (g_gate && there) store_row<V>(g_gate + row * p.channels, p, at.lane, dgate);
+            if (g_gate && there) store_row<V, E>(g_gate + row * p.channels, p, at.lane, dgate);
         }
-        if (g_branch && there) store_row<V>(g_branch + row * p.channels, p, at.lane, gx);
+        if (g_branch && there) store_row<V, E>(g_branch + row * p.channels, p, at.lane, gx);
     }
     // the groups of the workgroup one after another
     float *out = part + int64_t(blockIdx.x) * 2 * p.channels;
     for (int g = 0; g < at.groups; ++g) {
         if (at.group == g) {
-#pragma unroll
-            for (int j = 0; j < E / V; ++j) {
-#pragma unroll
-                for (int k = 0; k < V; ++k) {
-                    const int c = (j * p.lanes + at.lane) * V + k;
-                    if (c >= p.channels) continue;
-                    float both_c = sum_both[j * V + k], next_c = sum_next[j * V + k];
-                    if (g > 0) {
-                        both_c += sums[c];
-                        next_c += sums[p.channels + c];
-                    }
-                    if (g == at.groups - 1) {
-                        out[c] = both_c;
-                        out[p.channels + c] = next_c;
-                    } else {
-                        sums[c] = both_c;
-                        sums[p.channels + c] = next_c;
-                    }
+each_channel<V, E, N>(p, at.lane, [&](int c, int k) {
+                float both_c = sum_both[k], next_c = sum_next[k];
+                if (g > 0) {
+                    both_c += sums[c];
+                    next_c += sums[p.channels + c];
                 }
-            }
+                if (g == at.groups - 1) {
+                    out[c] = both_c;
+                    out[p.channels + c] = next_c;
+                } else {
+                    sums[c] = both_c;
+                    sums[p.channels + c] = next_c;
+                }
+            });
         }
         if (g < at.groups - 1) __syncthreads();
     }
@@ -353,13 +369,8 @@ static int check_norm_operands(const pesq_residual_norm *p) {
     return PESQ_OK;
 }
 
-static NormArgs norm_args(const pesq_residual_norm *p, int lanes) {
-    return {p->rows, p->channels, p->x, p->branch, p->gate, p->strides[0], p->strides[1],
-            p->strides[2], p->post_weight, p->scale, p->next_weight, static_cast<float>(p->eps), lanes};
-}
-
 // How rows are spread.  elements: of a thread; lanes: of a row, the fewest of a
-// power of two; vector: 16 byte moves.
+// power of two; whole: channels in whole 16 byte moves of the branch's type.
 //
 // The forward takes 16 elements above 512 channels, so that rows of up to 1024
 // stay in one wavefront and need no barrier: 60016 x 1024 (bfloat16 under a
@@ -367,8 +378,7 @@ static NormArgs norm_args(const pesq_residual_norm *p, int lanes) {
 // much and takes 8 up to 2048 channels (a quarter of a compute unit's registers
 // per wavefront then, half with 16): 259 us, against 296 us with 16.
 struct NormPlan {
-    int elements, lanes, threads;
-    bool vector;
+    int elements, lanes, threads, whole;
     int64_t passes(int64_t rows) const { return cdiv(rows, threads / lanes); }
 };
 
@@ -384,43 +394,39 @@ static int64_t bwd_workgroups(int64_t passes) {
     return half < kBwdWorkgroups ? half : kBwdWorkgroups;
 }
 
-static NormPlan norm_plan(const pesq_residual_norm *p, bool vector, int narrow) {
+static NormPlan norm_plan(const pesq_residual_norm *p, int narrow) {
     NormPlan plan;
     plan.elements = p->channels <= narrow ? 8 : 16;
-    plan.lanes = vector && plan.elements == 8 ? 16 : kWave;
-    while (int64_t(plan.lanes) * plan.elements < p->channels) plan.lanes *= 2;
+    plan.lanes = plan.elements == 8 ? 16 : kWave;
+    plan.whole = static_cast<int>(p->channels / (16 / type_size(p->dtype)) * (16 / type_size(p->dtype)));
+    while (plan.lanes * plan.elements < plan.whole) plan.lanes *= 2;
     plan.threads = plan.lanes > kNormThreads ? plan.lanes : kNormThreads;
-    plan.vector = vector;
     return plan;
 }
 
-// whether rows of `size` byte elements at p start at multiples of 16 bytes (p may be NULL)
-static bool rows_aligned(const void *p, int64_t stride, int size) {
-    return !p || (reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0);
+static NormArgs norm_args(const pesq_residual_norm *p, const NormPlan &plan) {
+    return {p->rows, p->channels, p->x, p->branch, p->gate, p->strides[0], p->strides[1],
+            p->strides[2], p->post_weight, p->scale, p->next_weight, static_cast<float>(p->eps), plan.lanes,
+            plan.whole};
 }
 
-static bool rows_vector(const pesq_residual_norm *p) {
-    const int wide = type_size(p->stream_dtype), size = type_size(p->dtype);
-    return p->channels % (16 / size) == 0 && rows_aligned(p->x, p->strides[0], wide) &&
-           rows_aligned(p->branch, p->strides[1], size) && rows_aligned(p->gate, p->strides[2], size);
-}
-
-// fn(V, E, width) as constants
+// fn(V, E, width, tail) as constants
 template <class T, class Fn>
-static void with_plan(const NormPlan &plan, Fn fn) {
+static void with_plan(const NormPlan &plan, bool tail, Fn fn) {
     using std::integral_constant;
-    constexpr int V = 16 / sizeof(T);
-    if (plan.vector) {
-        integral_constant<int, V> v;
-        if (plan.elements == 16) return fn(v, integral_constant<int, 16>(), integral_constant<int, 64>());
-        integral_constant<int, 8> e;
-        if (plan.lanes == 16) return fn(v, e, integral_constant<int, 16>());
-        if (plan.lanes == 32) return fn(v, e, integral_constant<int, 32>());
-        return fn(v, e, integral_constant<int, 64>());
-    }
-    integral_constant<int, 1> one;
-    if (plan.elements == 16) return fn(one, integral_constant<int, 16>(), integral_constant<int, 64>());
-    fn(one, integral_constant<int, 8>(), integral_constant<int, 64>());
+    const integral_constant<int, 16 / sizeof(T)> v;
+    const auto with_tail = [&](auto e, auto width) {
+        if (tail) {
+            fn(v, e, width, std::true_type());
+        } else {
+            fn(v, e, width, std::false_type());
+        }
+    };
+    const integral_constant<int, 8> e;
+    if (plan.elements == 16) return with_tail(integral_constant<int, 16>(), integral_constant<int, 64>());
+    if (plan.lanes == 16) return with_tail(e, integral_constant<int, 16>());
+    if (plan.lanes == 32) return with_tail(e, integral_constant<int, 32>());
+    with_tail(e, integral_constant<int, 64>());
 }
 
 // fn(S(), T()) with the stream's and the branch's types
@@ -451,18 +457,15 @@ extern "C" int pesq_residual_norm_forward(const pesq_residual_norm *p, void *x_o
     if (int st = check_norm_operands(p)) return st;
     if (p->rows == 0) return PESQ_OK;
     PESQ_CHECK_ARG((!p->branch || x_out) && (!p->next_weight || n_out), "null argument");
-    const int64_t channels = p->channels;
-    const NormPlan plan =
-        norm_plan(p, rows_vector(p) && rows_aligned(x_out, channels, type_size(p->stream_dtype)) &&
-                         rows_aligned(n_out, channels, type_size(p->dtype)), kFwdNarrow);
+    const NormPlan plan = norm_plan(p, kFwdNarrow);
     const unsigned grid = static_cast<unsigned>(fwd_workgroups(plan.passes(p->rows)));
     with_types(p, [&](auto s, auto t) {
         using S = decltype(s);
         using T = decltype(t);
-        with_plan<T>(plan, [&](auto v, auto e, auto width) {
-            residual_norm_fwd_kernel<S, T, v.value, e.value, width.value>
+        with_plan<T>(plan, plan.whole < p->channels, [&](auto v, auto e, auto width, auto tail) {
+            residual_norm_fwd_kernel<S, T, v.value, e.value, width.value, tail.value>
                 <<<grid, plan.threads, 0, stream>>>(
-                    norm_args(p, plan.lanes), static_cast<S *>(x_out), static_cast<T *>(n_out), inverse);
+                    norm_args(p, plan), static_cast<S *>(x_out), static_cast<T *>(n_out), inverse);
         });
     });
     PESQ_CHECK_LAUNCH("pesq_residual_norm_forward");
@@ -483,22 +486,18 @@ extern "C" int pesq_residual_norm_backward(const pesq_residual_norm *p, const vo
                    "a gradient is asked of an operand that is not there");
     PESQ_CHECK_ARG(!g_next || g_n_out || p->rows == 0, "the next weight's gradient without n's");
     PESQ_CHECK_ARG(!g_scale || p->post_weight, "null argument");
-    const int wide = type_size(p->stream_dtype), size = type_size(p->dtype);
     const int64_t channels = p->channels;
-    const NormPlan plan = norm_plan(
-        p, rows_vector(p) && rows_aligned(g_x_out, g_strides[0], wide) &&
-               rows_aligned(g_n_out, g_strides[1], size) && rows_aligned(g_x, channels, wide) &&
-               rows_aligned(g_branch, channels, size) && rows_aligned(g_gate, channels, size), kBwdNarrow);
+    const NormPlan plan = norm_plan(p, kBwdNarrow);
     float *part = static_cast<float *>(workspace);
     const int64_t parts = bwd_workgroups(plan.passes(p->rows));
     if (p->rows > 0) {
         with_types(p, [&](auto s, auto t) {
             using S = decltype(s);
             using T = decltype(t);
-            with_plan<T>(plan, [&](auto v, auto e, auto width) {
-                residual_norm_bwd_kernel<S, T, v.value, e.value, width.value>
+            with_plan<T>(plan, plan.whole < p->channels, [&](auto v, auto e, auto width, auto tail) {
+                residual_norm_bwd_kernel<S, T, v.value, e.value, width.value, tail.value>
                     <<<static_cast<unsigned>(parts), plan.threads, 0, stream>>>(
-                        norm_args(p, plan.lanes), static_cast<const S *>(g_x_out), g_strides[0],
+                        norm_args(p, plan), static_cast<const S *>(g_x_out), g_strides[0],
                         static_cast<const T *>(g_n_out), g_strides[1], inverse, static_cast<S *>(g_x),
                         static_cast<T *>(g_branch), static_cast<T *>(g_gate), part);
             });
