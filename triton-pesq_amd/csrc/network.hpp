@@ -71,4 +71,27 @@ __device__ __forceinline__ void store_neighbours(T *p, const Neighbours<T, V> &e
     for (int k = 0; k < kBytes / kMove; ++k) reinterpret_cast<Move *>(p)[k] = moves.m[k];
 }
 
+// Sums of columns of partial sums [parts][stride] by a workgroup of kSumShares
+// threads for each of kSumColumns columns: shares of the parts first, then their
+// sums pairwise in LDS.  Returns column `c`'s (c < columns) to the threads of
+// share 0.  Many shares, since the time is that of a thread's loads in a row.
+constexpr int kSumShares = 64, kSumColumns = 16;
+
+__device__ __forceinline__ float sum_parts(const float *part, int64_t parts, int64_t stride, int64_t c,
+                                           int64_t columns) {
+    __shared__ float sums[kSumShares][kSumColumns];
+    const int column = threadIdx.x % kSumColumns, share = threadIdx.x / kSumColumns;
+    float sum = 0.0f;
+    if (c < columns) {
+#pragma unroll 8
+        for (int64_t k = share; k < parts; k += kSumShares) sum += part[k * stride + c];
+    }
+    sums[share][column] = sum;
+    for (int half = kSumShares / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (share < half) sums[share][column] += sums[share + half][column];
+    }
+    return sums[0][column];
+}
+
 }  // namespace pesq

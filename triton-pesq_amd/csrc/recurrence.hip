@@ -547,25 +547,13 @@ __global__ void __launch_bounds__(kMaxWaves *kWave)
     }
 }
 
-// ddecay from the chunks' shares: kSumRows threads per channel, each a share of
-// the rows, joined in LDS
-constexpr int kSumRows = 16, kSumChannels = 64;
-__global__ void __launch_bounds__(kSumRows *kSumChannels)
+// ddecay from the chunks' shares
+__global__ void __launch_bounds__(kSumShares *kSumColumns)
     recurrence_decay_kernel(const float *part, int64_t rows, int64_t channels, const float *decay,
                             float rate, float *g_decay) {
-    __shared__ float sums[kSumRows][kSumChannels];
-    const int lane = threadIdx.x % kSumChannels, share = threadIdx.x / kSumChannels;
-    const int64_t c = int64_t(blockIdx.x) * kSumChannels + lane;
-    float sum = 0.0f;
-    if (c < channels) {
-#pragma unroll 8
-        for (int64_t k = share; k < rows; k += kSumRows) sum += part[k * channels + c];
-    }
-    sums[share][lane] = sum;
-    __syncthreads();
-    if (share != 0 || c >= channels) return;
-    for (int k = 1; k < kSumRows; ++k) sum += sums[k][lane];
-    g_decay[c] = sum * (rate * sigmoid_fast(decay[c]));
+    const int64_t c = int64_t(blockIdx.x) * kSumColumns + threadIdx.x % kSumColumns;
+    const float sum = sum_parts(part, rows, channels, c, channels);
+    if (threadIdx.x < kSumColumns && c < channels) g_decay[c] = sum * (rate * sigmoid_fast(decay[c]));
 }
 
 // kPending into all words, and open_log2 of every channel into rates
@@ -757,8 +745,8 @@ extern "C" int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_
         PESQ_CHECK_LAUNCH("pesq_recurrence_backward");
     }
     if (g_decay) {
-        recurrence_decay_kernel<<<static_cast<unsigned>(cdiv(p->channels, kSumChannels)),
-                                  kSumRows * kSumChannels, 0, stream>>>(
+        recurrence_decay_kernel<<<static_cast<unsigned>(cdiv(p->channels, kSumColumns)),
+                                  kSumShares * kSumColumns, 0, stream>>>(
             part, plan.chunks * p->batch, p->channels, p->decay, static_cast<float>(p->rate), g_decay);
         PESQ_CHECK_LAUNCH("pesq_recurrence_backward");
     }

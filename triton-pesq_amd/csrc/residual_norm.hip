@@ -32,7 +32,6 @@ namespace pesq {
 
 constexpr int kNormThreads = 256;  // (512 for rows of more than 4096 channels)
 constexpr int kMostNormThreads = 512;
-constexpr int kSumShares = 16, kSumColumns = 64;
 
 struct NormArgs {
     int64_t rows, channels;
@@ -314,23 +313,14 @@ each_channel<V, E, N>(p, at.lane, [&](int c, int k) {
 }
 
 // the weights' gradients (NULL: not asked for) from the partial sums: blockIdx.y 0
-// post and scale, 1 next; kSumShares threads a column, joined in LDS
+// post and scale, 1 next
 __global__ void __launch_bounds__(kSumShares *kSumColumns)
     residual_norm_sum_kernel(const float *part, int64_t parts, int64_t channels, const float *post,
                              const float *scale, float *g_post, float *g_scale, float *g_next) {
-    __shared__ float sums[kSumShares][kSumColumns];
-    const int column = threadIdx.x % kSumColumns, share = threadIdx.x / kSumColumns;
-    const int64_t c = int64_t(blockIdx.x) * kSumColumns + column;
     if (blockIdx.y == 1 ? !g_next : !g_post && !g_scale) return;
-    float sum = 0.0f;
-    if (c < channels) {
-#pragma unroll 8
-        for (int64_t k = share; k < parts; k += kSumShares) sum += part[(2 * k + blockIdx.y) * channels + c];
-    }
-    sums[share][column] = sum;
-    __syncthreads();
-    if (share != 0 || c >= channels) return;
-    for (int k = 1; k < kSumShares; ++k) sum += sums[k][column];
+    const int64_t c = int64_t(blockIdx.x) * kSumColumns + threadIdx.x % kSumColumns;
+    const float sum = sum_parts(part + blockIdx.y * channels, parts, 2 * channels, c, channels);
+    if (threadIdx.x >= kSumColumns || c >= channels) return;
     if (blockIdx.y == 1) {
         g_next[c] = sum;
     } else {
@@ -375,15 +365,16 @@ static int check_norm_operands(const pesq_residual_norm *p) {
 // The forward takes 16 elements above 512 channels, so that rows of up to 1024
 // stay in one wavefront and need no barrier: 60016 x 1024 (bfloat16 under a
 // float32 stream) 162 us, against 191 us with 8.  The backward holds twice as
-// much and takes 8 up to 2048 channels (a quarter of a compute unit's registers
-// per wavefront then, half with 16): 259 us, against 296 us with 16.
+// much and takes 8 up to 4096 channels (a quarter of a SIMD's registers per
+// wavefront then, half with 16): 259 us, against 296 us with 16; 9000 x 3104
+// bfloat16 with the forward 219 us, against 262 us.
 struct NormPlan {
     int elements, lanes, threads, whole;
     int64_t passes(int64_t rows) const { return cdiv(rows, threads / lanes); }
 };
 
 constexpr int64_t kFwdWorkgroups = 2048, kBwdWorkgroups = 1024;
-constexpr int kFwdNarrow = 8 * kWave, kBwdNarrow = 32 * kWave;
+constexpr int kFwdNarrow = 8 * kWave, kBwdNarrow = 64 * kWave;
 
 static int64_t fwd_workgroups(int64_t passes) { return passes < kFwdWorkgroups ? passes : kFwdWorkgroups; }
 
