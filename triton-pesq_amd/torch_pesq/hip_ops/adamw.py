@@ -62,12 +62,14 @@ class HipAdamW(torch.optim.Optimizer):
     def state_bits(self):
         return self.param_groups[0]["state_bits"]
 
+    @torch.no_grad()
     def _build(self):
         """Lay the moments of all parameters out, taking over what the state holds."""
 
         bits = self.state_bits
         plan = _lib.torch_ext().AdamWPlan([list(group["params"]) for group in self.param_groups], bits)
         steps, index = plan.steps(), 0
+        copies = {}
         for g, group in enumerate(self.param_groups):
             for k, p in enumerate(group["params"]):
                 views = dict(zip(_NAMES[bits], plan.views(g, k)), step=steps[index])
@@ -82,13 +84,18 @@ class HipAdamW(torch.optim.Optimizer):
                             f"`{name}` of a state of {bits} bits has to be {to.dtype} {tuple(to.shape)}, "
                             f"got {held.dtype} {tuple(held.shape)}."
                         )
-                    to.copy_(held)
+                    to_all, held_all = copies.setdefault(to.dtype, ([], []))
+                    to_all.append(to)
+                    held_all.append(held)
                 self.state[p] = views
+        for to_all, held_all in copies.values():
+            torch._foreach_copy_(to_all, held_all)
         self._plan = plan
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step of all parameters that have a gradient, on the current stream."""
+
+        # (nothing here is recorded for autograd, so no guard against it is entered)
 
         loss = None
         if closure is not None:
