@@ -13,7 +13,9 @@
  * last failure of the calling thread.
  *
  * Each function replaces the reference operator named in its comment
- * (paths relative to the LarocheC/triton-pesq source tree).
+ * (paths relative to the LarocheC/triton-pesq source tree).  The operators of the
+ * networks that the loss trains (last section) are additions: their tensors are
+ * float32, bfloat16 or float16 and may be strided.
  */
 #ifndef PESQ_HIP_H
 #define PESQ_HIP_H
