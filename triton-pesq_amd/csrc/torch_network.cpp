@@ -34,6 +34,11 @@ at::Tensor dense_rows(const at::Tensor &t) {
     return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
+// t itself where it has the type (`to` would cost a call's dispatch)
+at::Tensor of_type(const at::Tensor &t, at::ScalarType type) {
+    return t.scalar_type() == type ? t : t.to(type);
+}
+
 // the gradients, with a derivative that raises where a double backward would need one
 void mark_once(variable_list &grads, const variable_list &upstream) {
     bool needed = false;
@@ -110,39 +115,50 @@ at::Tensor recurrence_rows(const at::Tensor &t) {
     return t.stride(1) < (int64_t(1) << 26) ? dense_rows(t) : t.contiguous();
 }
 
+struct RecurrenceResult {
+    RecurrenceInputs in;
+    at::Tensor y, last, starts;
+};
+
+// keep: with the states that the backward reads
+RecurrenceResult run_recurrence(const at::Tensor &x, const at::Tensor &recur, const at::Tensor &input,
+                                const at::Tensor &decay, const OptTensor &initial,
+                                const OptTensor &reset, bool reverse, double rate, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    RecurrenceResult r;
+    r.in = {recurrence_rows(x), recurrence_rows(recur), recurrence_rows(input), decay.contiguous(),
+            initial ? initial->contiguous() : at::Tensor(), reset ? reset->contiguous() : at::Tensor()};
+    const pesq_recurrence p = r.in.call(reverse, rate);
+    size_t starts_bytes = 0, ws_bytes = 0;
+    check(pesq_recurrence_workspace(&p, &starts_bytes, &ws_bytes, nullptr),
+          "pesq_recurrence_workspace");
+    const auto bytes = x.options().dtype(at::kByte).requires_grad(false);
+    at::Tensor ws;
+    if (keep) r.starts = at::empty({static_cast<int64_t>(starts_bytes)}, bytes);
+    if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, bytes);
+    r.y = at::empty(x.sizes(), x.options());
+    r.last = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
+    check(pesq_recurrence_forward(&p, r.y.data_ptr(), r.last.data_ptr<float>(),
+                                  static_cast<float *>(data(r.starts)), data(ws), current_stream(x)),
+          "pesq_recurrence_forward");
+    return r;
+}
+
 struct Recurrence : public torch::autograd::Function<Recurrence> {
     static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &recur,
                                  const at::Tensor &input, const at::Tensor &decay,
                                  const OptTensor &initial, const OptTensor &reset, bool reverse,
-                                 double rate, bool keep) {
-        const c10::DeviceGuard guard(x.device());
-        RecurrenceInputs in{recurrence_rows(x), recurrence_rows(recur), recurrence_rows(input),
-                            decay.contiguous(), initial ? initial->contiguous() : at::Tensor(),
-                            reset ? reset->contiguous() : at::Tensor()};
-        const pesq_recurrence p = in.call(reverse, rate);
-        size_t starts_bytes = 0, ws_bytes = 0;
-        check(pesq_recurrence_workspace(&p, &starts_bytes, &ws_bytes, nullptr),
-              "pesq_recurrence_workspace");
-        const auto bytes = x.options().dtype(at::kByte);
-        at::Tensor starts, ws;
-        if (keep) starts = at::empty({static_cast<int64_t>(starts_bytes)}, bytes);
-        if (ws_bytes > 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, bytes);
-        at::Tensor y = at::empty(x.sizes(), x.options());
-        at::Tensor last = at::empty({x.size(0), x.size(2)}, x.options().dtype(at::kFloat));
-        check(pesq_recurrence_forward(&p, y.data_ptr(), last.data_ptr<float>(),
-                                      static_cast<float *>(data(starts)), data(ws), current_stream(x)),
-              "pesq_recurrence_forward");
+                                 double rate) {
+        const RecurrenceResult r = run_recurrence(x, recur, input, decay, initial, reset, reverse, rate, true);
         ctx->set_materialize_grads(false);
-        if (keep) {
-            ctx->save_for_backward({in.x, in.recur, in.input, in.decay, in.initial, in.reset, starts});
-            ctx->saved_data["reverse"] = reverse;
-            ctx->saved_data["rate"] = rate;
-        }
-        return {y, last};
+        ctx->save_for_backward({r.in.x, r.in.recur, r.in.input, r.in.decay, r.in.initial, r.in.reset, r.starts});
+        ctx->saved_data["reverse"] = reverse;
+        ctx->saved_data["rate"] = rate;
+        return {r.y, r.last};
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        variable_list out(9);
+        variable_list out(8);  // one per argument of forward
         if (!grads[0].defined() && !grads[1].defined()) return out;
         const variable_list saved = ctx->get_saved_variables();
         const RecurrenceInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5]};
@@ -156,8 +172,8 @@ struct Recurrence : public torch::autograd::Function<Recurrence> {
         at::Tensor g_y, g_last;
         {
             const at::NoGradGuard no_grad;
-            if (grads[0].defined()) g_y = recurrence_rows(grads[0].to(x.scalar_type()));
-            if (grads[1].defined()) g_last = grads[1].to(at::kFloat).contiguous();
+            if (grads[0].defined()) g_y = recurrence_rows(of_type(grads[0], x.scalar_type()));
+            if (grads[1].defined()) g_last = of_type(grads[1], at::kFloat).contiguous();
         }
         for (int k = 0; k < 3; ++k) {
             if (ctx->needs_input_grad(k)) out[k] = at::empty(x.sizes(), x.options());
@@ -193,7 +209,11 @@ std::vector<at::Tensor> gated_recurrence(const at::Tensor &x, const at::Tensor &
     const bool keep = torch::autograd::GradMode::is_enabled() &&
                       (x.requires_grad() || recur.requires_grad() || input.requires_grad() ||
                        decay.requires_grad() || (initial && initial->requires_grad()));
-    return Recurrence::apply(x, recur, input, decay, initial, reset, reverse, rate, keep);
+    if (keep) return Recurrence::apply(x, recur, input, decay, initial, reset, reverse, rate);
+    // (a call without a gradient is spared the node)
+    const at::NoGradGuard no_grad;
+    const RecurrenceResult r = run_recurrence(x, recur, input, decay, initial, reset, reverse, rate, false);
+    return {r.y, r.last};
 }
 
 at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
@@ -247,49 +267,58 @@ struct NormInputs {
     }
 };
 
+struct NormResult {
+    NormInputs in;
+    int32_t dtype;
+    at::Tensor inverse;
+    variable_list out;  // [x_out][n_out]
+};
+
+// dtype: of n where there is no branch; keep: with what the backward reads
+NormResult run_norm(const at::Tensor &x, const OptTensor &branch, const OptTensor &gate,
+                    const OptTensor &post, const OptTensor &scale, const OptTensor &next,
+                    int64_t dtype, double eps, bool keep) {
+    const c10::DeviceGuard guard(x.device());
+    const int64_t channels = x.size(-1), rows = channels ? x.numel() / channels : 0;
+    const auto rows_of = [&](const OptTensor &t) {
+        return t ? as_rows(*t, rows, channels) : at::Tensor();
+    };
+    const auto weight = [](const OptTensor &t) { return t ? t->contiguous() : at::Tensor(); };
+    NormResult r;
+    r.in = {rows_of(x), rows_of(branch), rows_of(gate), weight(post), weight(scale), weight(next)};
+    pesq_residual_norm p = r.in.call(eps);
+    if (!branch) p.dtype = static_cast<int32_t>(dtype);
+    r.dtype = p.dtype;
+    const at::ScalarType typed = p.dtype == PESQ_F32    ? at::kFloat
+                                 : p.dtype == PESQ_BF16 ? at::kBFloat16
+                                                        : at::kHalf;
+    at::Tensor x_out, n_out;
+    if (branch) r.out.push_back(x_out = at::empty(x.sizes(), x.options()));
+    if (next) r.out.push_back(n_out = at::empty(x.sizes(), x.options().dtype(typed)));
+    if (keep) r.inverse = at::empty({rows, 2}, x.options().dtype(at::kFloat));
+    check(pesq_residual_norm_forward(&p, data(x_out), data(n_out), data_or_null<float>(r.inverse),
+                                     current_stream(x)),
+          "pesq_residual_norm_forward");
+    return r;
+}
+
 struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
-    // variables: x, branch, gate, post, scale, next; dtype: of n where there is no branch
+    // variables: x, branch, gate, post, scale, next
     static variable_list forward(AutogradContext *ctx, const at::Tensor &x, const OptTensor &branch,
                                  const OptTensor &gate, const OptTensor &post,
                                  const OptTensor &scale, const OptTensor &next, int64_t dtype,
-                                 double eps, bool keep) {
-        const c10::DeviceGuard guard(x.device());
-        const int64_t channels = x.size(-1), rows = channels ? x.numel() / channels : 0;
-        const auto rows_of = [&](const OptTensor &t) {
-            return t ? as_rows(*t, rows, channels) : at::Tensor();
-        };
-        const auto weight = [](const OptTensor &t) { return t ? t->contiguous() : at::Tensor(); };
-        const NormInputs in{rows_of(x), rows_of(branch), rows_of(gate),
-                            weight(post), weight(scale), weight(next)};
-        pesq_residual_norm p = in.call(eps);
-        if (!branch) p.dtype = static_cast<int32_t>(dtype);
-        const auto of_type = [&](int code) {
-            return x.options().dtype(code == PESQ_F32    ? at::kFloat
-                                     : code == PESQ_BF16 ? at::kBFloat16
-                                                         : at::kHalf);
-        };
-        at::Tensor x_out, n_out, inverse;
-        if (branch) x_out = at::empty(x.sizes(), x.options());
-        if (next) n_out = at::empty(x.sizes(), of_type(p.dtype));
-        if (keep) inverse = at::empty({rows, 2}, x.options().dtype(at::kFloat));
-        check(pesq_residual_norm_forward(&p, data(x_out), data(n_out), data_or_null<float>(inverse),
-                                         current_stream(x)),
-              "pesq_residual_norm_forward");
+                                 double eps) {
+        const NormResult r = run_norm(x, branch, gate, post, scale, next, dtype, eps, true);
         ctx->set_materialize_grads(false);
-        if (keep) {
-            ctx->save_for_backward({in.x, in.branch, in.gate, in.post, in.scale, in.next, inverse});
-            ctx->saved_data["eps"] = eps;
-            ctx->saved_data["dtype"] = static_cast<int64_t>(p.dtype);
-            ctx->saved_data["sizes"] = x.sizes().vec();
-        }
-        variable_list out;
-        if (x_out.defined()) out.push_back(x_out);
-        if (n_out.defined()) out.push_back(n_out);
-        return out;
+        ctx->save_for_backward({r.in.x, r.in.branch, r.in.gate, r.in.post, r.in.scale, r.in.next, r.inverse});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["dtype"] = static_cast<int64_t>(r.dtype);
+        ctx->saved_data["sizes"] = x.sizes().vec();
+        return r.out;
     }
 
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
-        variable_list out(9);
+        variable_list out(8);  // one per argument of forward
         const variable_list saved = ctx->get_saved_variables();
         const NormInputs in{saved[0], saved[1], saved[2], saved[3], saved[4], saved[5]};
         at::Tensor g_x_out, g_n_out;
@@ -303,7 +332,7 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         {
             const at::NoGradGuard no_grad;
             if (g_x_out.defined()) {
-                g_x_out = as_rows(g_x_out.to(in.x.scalar_type()), p.rows, p.channels);
+                g_x_out = as_rows(of_type(g_x_out, in.x.scalar_type()), p.rows, p.channels);
             }
             if (g_n_out.defined()) g_n_out = as_rows(g_n_out, p.rows, p.channels);
         }
@@ -378,14 +407,17 @@ std::vector<at::Tensor> residual_norm(const at::Tensor &x, const OptTensor &bran
     check_weight(post, "weight", x);
     check_weight(scale, "scale", x);
     check_weight(next, branch ? "next_weight" : "weight", x);
-    const auto f32 = [](const OptTensor &t) { return t ? OptTensor(t->to(at::kFloat)) : t; };
+    const auto f32 = [](const OptTensor &t) { return t ? OptTensor(of_type(*t, at::kFloat)) : t; };
     const OptTensor w = f32(post), s = f32(scale), n = f32(next);
     bool keep = x.requires_grad();
     for (const OptTensor *t : std::array<const OptTensor *, 5>{&branch, &gate, &w, &s, &n}) {
         keep = keep || (*t && (*t)->requires_grad());
     }
-    return ResidualNorm::apply(x, branch, gate, w, s, n, code, eps,
-                               keep && torch::autograd::GradMode::is_enabled());
+    if (keep && torch::autograd::GradMode::is_enabled()) {
+        return ResidualNorm::apply(x, branch, gate, w, s, n, code, eps);
+    }
+    const at::NoGradGuard no_grad;
+    return run_norm(x, branch, gate, w, s, n, code, eps, false).out;
 }
 
 // ---------------------------------------------------------------------------
