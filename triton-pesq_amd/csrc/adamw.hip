@@ -5,9 +5,8 @@
 //
 // in float32, each product and sum rounded as written (no fused steps), so that
 // the moments are those of the same formula in plain float32 operations.
-// Elementwise, so bound by memory with 32 bit moments, and by both memory and
-// arithmetic with 8 (47.7 M bfloat16 weights: 122 us, 3.9 TB/s, 95 us of which
-// the vector units issue).
+// Elementwise and bound by memory (47.7 M bfloat16 weights with 8 bit moments:
+// 96 to 105 us by card, 4.5 to 5.0 TB/s, the rate of a large copy).
 //
 // 8 bit moments are held in blocks of 256 elements of one tensor, each with its
 // largest magnitude as a float32 scale, and per element the nearest
@@ -38,12 +37,20 @@ struct AdamArgs {
 
 // A launch takes up to kTensors tensors as kernel arguments: no table to copy to
 // the GPU, and new gradients each step cost nothing.  Workgroups go by tiles of
-// kTile elements; a tile's tensor is found by bisection.
+// kAdamThreads lanes; a tile's tensor is found by bisection.
 constexpr int kTensors = 96;
-constexpr int kTileBlocks = 8;  // two for each wavefront
-constexpr int kTile = kTileBlocks * kBlock;
 constexpr int kAdamThreads = 256;
-constexpr int kLane = kBlock / kWave;  // neighbours of a block in a lane
+
+// Neighbours that a lane takes.  With 8 bit moments 8, a block to each half of a
+// wavefront: fewer and wider moves, and the scales' maxima and reciprocals shared
+// by more (47.7 M bfloat16 parameters 96 us; with 4 121 us, with 16, and half the
+// wavefronts at a time, 105 us).  With float32 moments 4, a move of 16 bytes that
+// continues its neighbour lane's (26 tensors, 1.4 M parameters, 9.1 us; with 8
+// 10.3 us), as in the kernel that writes the moments' values (76 us; 85 us).
+constexpr int lane_elements(bool eight) { return eight ? 8 : 4; }
+constexpr int tile_elements(bool eight) { return lane_elements(eight) * kAdamThreads; }
+constexpr int kHalfLane = kBlock / (kWave / 2);
+static_assert(lane_elements(true) == kHalfLane, "block_scale joins the halves of wavefronts");
 
 struct AdamTensor {
     void *param;
@@ -75,62 +82,70 @@ __device__ __forceinline__ float adamw(float p, float g, float &m, float &v, con
     return p * a.keep - update * a.step_size;
 }
 
-// what four bytes of codes stand for
-__device__ __forceinline__ void values(uint32_t cm, uint32_t cv, float sm, float sv, float (&m)[kLane],
-                                       float (&v)[kLane]) {
-    cm ^= 0x80808080u;
+// a lane's codes, and its moments in float32
+template <int E>
+struct alignas(E) Codes {
+    uint32_t v[E / 4];
+};
+template <int E>
+struct alignas(16) Lane {
+    float v[E];
+};
+
+// what the codes stand for
+template <int E>
+__device__ __forceinline__ void values(const Codes<E> &cm, const Codes<E> &cv, float sm, float sv, Lane<E> &m,
+                                       Lane<E> &v) {
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-        const float part = (static_cast<float>(cm >> 8 * k & 0xff) - 128.0f) * (1.0f / 127.0f);
-        m[k] = fabsf(part) * part * sm;
-        float root = static_cast<float>(cv >> 8 * k & 0xff) * (1.0f / 255.0f);
+    for (int k = 0; k < E; ++k) {
+        const float part =
+            (static_cast<float>((cm.v[k / 4] ^ 0x80808080u) >> 8 * (k % 4) & 0xff) - 128.0f) * (1.0f / 127.0f);
+        m.v[k] = fabsf(part) * part * sm;
+        float root = static_cast<float>(cv.v[k / 4] >> 8 * (k % 4) & 0xff) * (1.0f / 255.0f);
         root = root * root;
-        v[k] = root * root * sv;
+        v.v[k] = root * root * sv;
     }
 }
-
-struct alignas(16) Lane {
-    float v[kLane];
-};
 
 // Codes are those of correctly rounded roots.  The hardware's root (one unit in
 // the last place) gives the same code unless the product lies next to the middle
 // between two: within 127 2^-22 of it for the first moment and 255 2^-22 for the
-// second's two roots, twice the errors that can arise.  A block with such an
-// element, one in twenty, is done again.
+// second's two roots, twice the errors that can arise.  A wavefront with such an
+// element, one in ten, does its codes again.
 
 // the middle between two codes, seen from a number of codes
 __device__ __forceinline__ bool near_middle(float q, float distance) {
     return fabsf(__builtin_amdgcn_fractf(q) - 0.5f) <= distance;
 }
 
-// Bytes of four lane elements: int8 and uint8 codes.  A number of codes is
+// Bytes of a lane's elements: int8 and uint8 codes.  A number of codes is
 // rounded to the nearest one and clamped by the conversion that packs it; the
 // first moment's are 128 up while they are packed.
-template <bool kExact>
-__device__ __forceinline__ bool codes(const float (&m)[kLane], const float (&v)[kLane], float im, float iv,
-                                      uint32_t &cm, uint32_t &cv) {
+template <bool kExact, int E>
+__device__ __forceinline__ bool codes(const Lane<E> &m, const Lane<E> &v, float im, float iv, Codes<E> &cm,
+                                      Codes<E> &cv) {
     bool near = false;
     const float least = iv == 0.0f ? 0.0f : 1.0f;
-    cm = cv = 0;
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-        const float ym = fabsf(m[k]) * im, yv = v[k] * iv;
+    for (int k = 0; k < E; ++k) {
+        uint32_t &word_m = cm.v[k / 4], &word_v = cv.v[k / 4];
+        if (k % 4 == 0) word_m = word_v = 0;
+        const float ym = fabsf(m.v[k]) * im, yv = v.v[k] * iv;
         float qm, qv;
         if (kExact) {
-            qm = 128.0f + copysignf(rintf(sqrtf(ym) * 127.0f), m[k]);
+            qm = 128.0f + copysignf(rintf(sqrtf(ym) * 127.0f), m.v[k]);
             qv = rintf(sqrtf(sqrtf(yv)) * 255.0f);
         } else {
-            qm = fmaf(copysignf(__builtin_amdgcn_sqrtf(ym), m[k]), 127.0f, 128.0f);
+            qm = fmaf(copysignf(__builtin_amdgcn_sqrtf(ym), m.v[k]), 127.0f, 128.0f);
             qv = __builtin_amdgcn_sqrtf(__builtin_amdgcn_sqrtf(yv)) * 255.0f;
             const bool near_m = near_middle(qm, 127.0f * 0x1p-22f), near_v = near_middle(qv, 255.0f * 0x1p-22f);
             near = near | near_m | near_v;  // (no branch between elements)
         }
-        qv = fmaxf(qv, v[k] > 0.0f ? least : 0.0f);
-        cm = __builtin_amdgcn_cvt_pk_u8_f32(qm, k, cm);
-        cv = __builtin_amdgcn_cvt_pk_u8_f32(qv, k, cv);
+        qv = fmaxf(qv, v.v[k] > 0.0f ? least : 0.0f);
+        word_m = __builtin_amdgcn_cvt_pk_u8_f32(qm, k % 4, word_m);
+        word_v = __builtin_amdgcn_cvt_pk_u8_f32(qv, k % 4, word_v);
+        if (k % 4 == 3) word_m ^= 0x80808080u;
     }
-    cm ^= 0x80808080u;
     return near;
 }
 
@@ -141,24 +156,21 @@ __device__ __forceinline__ uint32_t max_ror(uint32_t v) {
     return other > v ? other : v;
 }
 
-// largest magnitude of a wavefront's block, NaN above all (its bits are the
-// largest); 0 where it is too small to be held
-__device__ __forceinline__ float block_scale(const float (&f)[kLane]) {
+// largest magnitude of the block in a half of a wavefront, NaN above all (its bits
+// are the largest); 0 where it is too small to be held
+__device__ __forceinline__ float block_scale(const Lane<kHalfLane> &f) {
     uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < kLane; ++k) {
-        const uint32_t other = __float_as_uint(f[k]) & 0x7fffffffu;
+    for (int k = 0; k < kHalfLane; ++k) {
+        const uint32_t other = __float_as_uint(f.v[k]) & 0x7fffffffu;
         bits = other > bits ? other : bits;
     }
     bits = max_ror<0x128>(bits);  // row_ror:8, 4, 2, 1
     bits = max_ror<0x124>(bits);
     bits = max_ror<0x122>(bits);
     bits = max_ror<0x121>(bits);
-    const auto row = [&](int lane) {
-        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits), lane));
-    };
-    const uint32_t low = row(0) > row(16) ? row(0) : row(16), high = row(32) > row(48) ? row(32) : row(48);
-    bits = low > high ? low : high;
+    const auto rows = __builtin_amdgcn_permlane16_swap(bits, bits, false, false);  // of the half
+    bits = rows[0] > rows[1] ? rows[0] : rows[1];
     const float scale = __uint_as_float(bits);
     return scale < kSmallest ? 0.0f : scale;
 }
@@ -166,29 +178,29 @@ __device__ __forceinline__ float block_scale(const float (&f)[kLane]) {
 __device__ __forceinline__ float inverse_of(float scale) { return scale == 0.0f ? 0.0f : 1.0f / scale; }
 
 // a lane's neighbours from element `at` of a tensor; zeros past its end
-template <class T>
-__device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count, float (&out)[kLane]) {
-    if (at + kLane <= count) {
-        const auto e = load_neighbours<T, kLane>(p + at);
+template <int E, class T>
+__device__ __forceinline__ void load_lane(const T *p, int64_t at, int64_t count, Lane<E> &out) {
+    if (at + E <= count) {
+        const auto e = load_neighbours<T, E>(p + at);
 #pragma unroll
-        for (int k = 0; k < kLane; ++k) out[k] = static_cast<float>(e.v[k]);
+        for (int k = 0; k < E; ++k) out.v[k] = static_cast<float>(e.v[k]);
     } else {
 #pragma unroll
-        for (int k = 0; k < kLane; ++k) out[k] = at + k < count ? static_cast<float>(p[at + k]) : 0.0f;
+        for (int k = 0; k < E; ++k) out.v[k] = at + k < count ? static_cast<float>(p[at + k]) : 0.0f;
     }
 }
 
-template <class T>
-__device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, const float (&f)[kLane]) {
-    if (at + kLane <= count) {
-        Neighbours<T, kLane> e;
+template <int E, class T>
+__device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, const Lane<E> &f) {
+    if (at + E <= count) {
+        Neighbours<T, E> e;
 #pragma unroll
-        for (int k = 0; k < kLane; ++k) e.v[k] = static_cast<T>(f[k]);
-        store_neighbours<T, kLane>(p + at, e);
+        for (int k = 0; k < E; ++k) e.v[k] = static_cast<T>(f.v[k]);
+        store_neighbours<T, E>(p + at, e);
     } else {
 #pragma unroll
-        for (int k = 0; k < kLane; ++k) {
-            if (at + k < count) p[at + k] = static_cast<T>(f[k]);
+        for (int k = 0; k < E; ++k) {
+            if (at + k < count) p[at + k] = static_cast<T>(f.v[k]);
         }
     }
 }
@@ -197,7 +209,7 @@ __device__ __forceinline__ void store_lane(T *p, int64_t at, int64_t count, cons
 // and stay 0.
 template <class T, bool kEight>
 __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
-    constexpr int kMine = kTileBlocks / (kAdamThreads / kWave);  // blocks of a wavefront
+    constexpr int E = lane_elements(kEight), kRow = kBlock / E;  // kRow lanes to a block
     int low = 0, high = list.count - 1;
     while (low < high) {
         const int middle = (low + high) / 2;
@@ -209,77 +221,53 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     }
     const AdamTensor &t = list.tensors[low];
     const uint32_t tile = blockIdx.x - (low ? list.tensors[low - 1].end : 0);
-    const int lane = lane_id();
-    const int64_t count = t.count, block0 = int64_t(tile) * kTileBlocks + wave_index() * kMine;
+    const int64_t at = (int64_t(tile) * kAdamThreads + threadIdx.x) * E, count = t.count;
+    if (at / kBlock * kBlock >= count) return;  // (all lanes of a block)
     T *param = static_cast<T *>(t.param);
     const T *grad = static_cast<const T *>(t.grad);
     const AdamArgs a = list.args;
-
-    float p[kMine][kLane], g[kMine][kLane], m[kMine][kLane], v[kMine][kLane];
-#pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-        const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
-        if (block * kBlock >= count) break;
-        load_lane(param, at, count, p[n]);
-        load_lane(grad, at, count, g[n]);
-        const int64_t held = int64_t(t.block) + block;
-        if constexpr (kEight) {
-            values(static_cast<const uint32_t *>(list.m)[held * kWave + lane],
-                   static_cast<const uint32_t *>(list.v)[held * kWave + lane], list.m_scale[held],
-                   list.v_scale[held], m[n], v[n]);
-        } else {
-            const Lane em = static_cast<const Lane *>(list.m)[held * kWave + lane];
-            const Lane ev = static_cast<const Lane *>(list.v)[held * kWave + lane];
-#pragma unroll
-            for (int k = 0; k < kLane; ++k) {
-                m[n][k] = em.v[k];
-                v[n][k] = ev.v[k];
-            }
-        }
+    const int64_t held = t.block + at / kBlock, mine = int64_t(t.block) * kRow + at / E;
+    Lane<E> p, g, m, v;
+    load_lane(param, at, count, p);
+    load_lane(grad, at, count, g);
+    if constexpr (kEight) {
+        values(static_cast<const Codes<E> *>(list.m)[mine], static_cast<const Codes<E> *>(list.v)[mine],
+               list.m_scale[held], list.v_scale[held], m, v);
+    } else {
+        m = static_cast<const Lane<E> *>(list.m)[mine];
+        v = static_cast<const Lane<E> *>(list.v)[mine];
     }
+    // (past the end m, v and g are 0, and the moments stay 0)
 #pragma unroll
-    for (int n = 0; n < kMine; ++n) {
-        const int64_t block = block0 + n, at = block * kBlock + lane * kLane;
-        if (block * kBlock >= count) break;
-        // (past the end m, v and g are 0, and the moments stay 0)
-#pragma unroll
-        for (int k = 0; k < kLane; ++k) p[n][k] = adamw(p[n][k], g[n][k], m[n][k], v[n][k], a);
-        store_lane(param, at, count, p[n]);
-        const int64_t held = int64_t(t.block) + block;
-        if constexpr (kEight) {
-            const float sm = block_scale(m[n]), sv = block_scale(v[n]);
-            const float im = inverse_of(sm), iv = inverse_of(sv);
-            uint32_t cm, cv;
-            if (__any(codes<false>(m[n], v[n], im, iv, cm, cv))) codes<true>(m[n], v[n], im, iv, cm, cv);
-            static_cast<uint32_t *>(list.m)[held * kWave + lane] = cm;
-            static_cast<uint32_t *>(list.v)[held * kWave + lane] = cv;
-            if (lane == 0) {
-                list.m_scale[held] = sm;
-                list.v_scale[held] = sv;
-            }
-        } else {
-            Lane em, ev;
-#pragma unroll
-            for (int k = 0; k < kLane; ++k) {
-                em.v[k] = m[n][k];
-                ev.v[k] = v[n][k];
-            }
-            static_cast<Lane *>(list.m)[held * kWave + lane] = em;
-            static_cast<Lane *>(list.v)[held * kWave + lane] = ev;
+    for (int k = 0; k < E; ++k) p.v[k] = adamw(p.v[k], g.v[k], m.v[k], v.v[k], a);
+    store_lane(param, at, count, p);
+    if constexpr (kEight) {
+        const float sm = block_scale(m), sv = block_scale(v);
+        const float im = inverse_of(sm), iv = inverse_of(sv);
+        Codes<E> cm, cv;
+        if (__any(codes<false>(m, v, im, iv, cm, cv))) codes<true>(m, v, im, iv, cm, cv);
+        static_cast<Codes<E> *>(list.m)[mine] = cm;
+        static_cast<Codes<E> *>(list.v)[mine] = cv;
+        if (at % kBlock == 0) {
+            list.m_scale[held] = sm;
+            list.v_scale[held] = sv;
         }
+    } else {
+        static_cast<Lane<E> *>(list.m)[mine] = m;
+        static_cast<Lane<E> *>(list.v)[mine] = v;
     }
 }
 
+constexpr int kValues = 4;  // of a lane
 __global__ void __launch_bounds__(kAdamThreads)
-    adamw_moments_kernel(const uint32_t *m, const uint32_t *v, const float *m_scale,
-                         const float *v_scale, int64_t blocks, float *m_out, float *v_out) {
-    const int64_t block = int64_t(blockIdx.x) * (kAdamThreads / kWave) + wave_index();
+    adamw_moments_kernel(const Codes<kValues> *m, const Codes<kValues> *v, const float *m_scale,
+                         const float *v_scale, int64_t blocks, Lane<kValues> *m_out, Lane<kValues> *v_out) {
+    const int64_t mine = int64_t(blockIdx.x) * kAdamThreads + threadIdx.x, block = mine * kValues / kBlock;
     if (block >= blocks) return;
-    const int64_t at = block * kWave + lane_id();
-    Lane em, ev;
-    values(m[at], v[at], m_scale[block], v_scale[block], em.v, ev.v);
-    reinterpret_cast<Lane *>(m_out)[at] = em;
-    reinterpret_cast<Lane *>(v_out)[at] = ev;
+    Lane<kValues> em, ev;
+    values(m[mine], v[mine], m_scale[block], v_scale[block], em, ev);
+    m_out[mine] = em;
+    v_out[mine] = ev;
 }
 
 // the launch of a list of `tiles` tiles
@@ -310,6 +298,7 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
     PESQ_CHECK_ARG(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0,
                    "betas have to be in [0, 1)");
     const bool eight = o->state_bits == 8;
+    const int64_t tile = tile_elements(eight);
     PESQ_CHECK_ARG(count == 0 || (exp_avg && exp_avg_sq && (!eight || (exp_avg_scale && exp_avg_sq_scale))),
                    "null argument");
     for (const void *array : {exp_avg, exp_avg_sq}) {
@@ -319,7 +308,7 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
         PESQ_CHECK_ARG(tensors[k].count >= 0 && tensors[k].first >= 0 && tensors[k].first % kBlock == 0,
                        "tensor %lld has no place in the moments", (long long)k);
         PESQ_CHECK_ARG(tensors[k].count == 0 || (tensors[k].param && tensors[k].grad), "null argument");
-        PESQ_CHECK_ARG(tensors[k].count <= kMostTiles * kTile && tensors[k].first < (int64_t(1) << 40),
+        PESQ_CHECK_ARG(tensors[k].count <= kMostTiles * tile && tensors[k].first < (int64_t(1) << 40),
                        "tensor %lld is too large", (long long)k);
     }
     const double step = static_cast<double>(o->step);
@@ -340,7 +329,7 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
     for (int64_t k = 0; k < count; ++k) {
         const pesq_adamw_tensor &t = tensors[k];
         if (t.count == 0) continue;
-        const int64_t more = cdiv(t.count, kTile);
+        const int64_t more = cdiv(t.count, tile);
         if (list.count == kTensors || tiles + more > kMostTiles) {
             launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
             PESQ_CHECK_LAUNCH("pesq_adamw_step");
@@ -369,9 +358,9 @@ extern "C" int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq,
         PESQ_CHECK_ARG(reinterpret_cast<uintptr_t>(array) % 16 == 0, "the moments start at multiples of 16 bytes");
     }
     const int64_t blocks = count / kBlock;
-    adamw_moments_kernel<<<static_cast<unsigned>(cdiv(blocks, kAdamThreads / kWave)), kAdamThreads, 0, stream>>>(
-        static_cast<const uint32_t *>(exp_avg), static_cast<const uint32_t *>(exp_avg_sq), exp_avg_scale,
-        exp_avg_sq_scale, blocks, m, v);
+    adamw_moments_kernel<<<static_cast<unsigned>(cdiv(count, kAdamThreads * kValues)), kAdamThreads, 0, stream>>>(
+        static_cast<const Codes<kValues> *>(exp_avg), static_cast<const Codes<kValues> *>(exp_avg_sq), exp_avg_scale,
+        exp_avg_sq_scale, blocks, reinterpret_cast<Lane<kValues> *>(m), reinterpret_cast<Lane<kValues> *>(v));
     PESQ_CHECK_LAUNCH("pesq_adamw_moments");
     return PESQ_OK;
 }
