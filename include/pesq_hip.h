@@ -520,8 +520,8 @@ int pesq_epilogue_backward(const float *d_symm, const float *d_asymm, const floa
  * batch item and per step, of x, recur_gate and input_gate; channels lie next
  * to each other.  decay [channels], initial [batch, channels] (NULL = 0) and
  * reset [batch, time] (NULL = none) are contiguous.  At most 65535 batch
- * items, 2^24 channels, 2^32 steps and 2^26 elements between two steps.  No
- * counterpart in the reference. */
+ * items, 2^24 channels and 2^32 steps, which start less than 2^27 bytes apart.
+ * No counterpart in the reference. */
 typedef struct pesq_recurrence {
     int64_t batch, time, channels;
     int32_t dtype; /* of x, the gates, y and their gradients */

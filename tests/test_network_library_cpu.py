@@ -157,3 +157,22 @@ def test_module_decay_spans_the_asked_memory():
     module = HipGatedRecurrence(1000, rate=4.0, fastest=0.5, slowest=0.99)
     open_gate = torch.exp(-4.0 * torch.nn.functional.softplus(module.decay.detach().double()))
     assert 0.4999 < float(open_gate.min()) < 0.52 and 0.97 < float(open_gate.max()) < 0.9901
+
+
+@pytest.mark.parametrize("dtype,most", [(0, 2**25), (1, 2**26), (2, 2**26)])
+def test_recurrence_steps_apart_in_bytes(dtype, most):
+    """The byte offset of a part's last row, 15 steps from its first, stays below 2^31."""
+
+    lib, size = _lib.library(), ctypes.c_size_t()
+    assert 15 * (most - 1) * (2 if dtype else 4) < 2**31
+    for tensor in range(3):
+        p = _recurrence(dtype=dtype)
+        p.strides[tensor][1] = most - 1
+        assert lib.pesq_recurrence_workspace(p, size, size, size) == 0
+        p.strides[tensor][1] = most
+        assert lib.pesq_recurrence_workspace(p, size, size, size) == 1 and "apart" in _message()
+    # the upstream gradient's
+    p = _recurrence(dtype=dtype, batch=0)
+    for stride, status in ((most - 1, 0), (most, 1)):
+        strides = (ctypes.c_int64 * 2)(0, stride)
+        assert lib.pesq_recurrence_backward(p, ANY, strides, None, ANY, None, None, None, None, ANY, ANY, None) == status

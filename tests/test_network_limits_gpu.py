@@ -54,6 +54,22 @@ def test_recurrence_rows_far_apart():
               _recurrence_step(part, decay, up[:1, :60].contiguous()))
 
 
+def test_recurrence_float32_steps_far_apart():
+    """Below 2^27 bytes apart as they are, from there on copied; both directions."""
+
+    t, decay, up = _recurrence_inputs((1, 60, 70), torch.float32)
+    far = torch.zeros(60 * (2**25 + 2), device="cuda")
+    for stride in (2**25 - 2, 2**25 + 2):
+        steps = far.as_strided((1, 60, 70), (0, stride, 1))
+        steps.copy_(t[1])
+        _same(_recurrence_step([t[0], steps, t[2]], decay, up), _recurrence_step(t, decay, up))
+        for reverse in (False, True):
+            _same([gated_recurrence(t[0], steps, t[2], decay, reverse=reverse)[0]],
+                  [gated_recurrence(*t, decay, reverse=reverse)[0]])
+        steps.copy_(up)
+        _same(_recurrence_step(t, decay, steps), _recurrence_step(t, decay, up))
+
+
 def test_recurrence_larger_than_32_bits():
     """More than 2^31 elements of y: the last rows against the same rows alone."""
 

@@ -581,8 +581,11 @@ __global__ void __launch_bounds__(kRecThreads) recurrence_step_kernel(RecArgs p,
 // host side
 // ---------------------------------------------------------------------------
 
-// so that the offsets of a part's rows stay below 2^31 bytes
-constexpr int64_t kMostStride = int64_t(1) << 26;
+// in bytes, so that the offset of a part's last row stays below 2^31
+constexpr int64_t kMostStride = int64_t(1) << 27;
+static_assert((kSteps - 1) * kMostStride <= kBufferBytes);
+
+static bool near_steps(int64_t stride, int dtype) { return stride < kMostStride / type_size(dtype); }
 
 static int check_recurrence(const pesq_recurrence *p) {
     PESQ_CHECK_ARG(p != nullptr, "null argument");
@@ -598,8 +601,8 @@ static int check_recurrence(const pesq_recurrence *p) {
     PESQ_CHECK_ARG(p->rate > 0.0 && std::isfinite(p->rate), "the rate has to be positive and finite");
     for (int k = 0; k < 6; ++k) {
         PESQ_CHECK_ARG(p->strides[k / 2][k % 2] >= 0, "negative stride");
-        PESQ_CHECK_ARG(k % 2 == 0 || p->strides[k / 2][1] < kMostStride,
-                       "steps are at most 2^26 elements apart, got %lld", (long long)p->strides[k / 2][1]);
+        PESQ_CHECK_ARG(k % 2 == 0 || near_steps(p->strides[k / 2][1], p->dtype),
+                       "steps are less than 2^27 bytes apart, got %lld elements", (long long)p->strides[k / 2][1]);
     }
     return PESQ_OK;
 }
@@ -722,7 +725,8 @@ extern "C" int pesq_recurrence_backward(const pesq_recurrence *p, const void *g_
                                         void *g_input, float *g_decay, float *g_initial,
                                         void *workspace, hipStream_t stream) {
     if (int st = check_operands(p)) return st;
-    PESQ_CHECK_ARG(!g_y || (g_strides && g_strides[0] >= 0 && g_strides[1] >= 0 && g_strides[1] < kMostStride),
+    PESQ_CHECK_ARG(!g_y || (g_strides && g_strides[0] >= 0 && g_strides[1] >= 0 &&
+                            near_steps(g_strides[1], p->dtype)),
                    "the upstream gradient needs its strides");
     if (p->channels == 0) return PESQ_OK;
     PESQ_CHECK_ARG(empty(p) || (workspace && (starts || p->time == 0)), "null argument");

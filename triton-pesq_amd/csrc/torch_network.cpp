@@ -112,7 +112,7 @@ void check_state(const at::Tensor &state, const char *name, const at::Tensor &x)
 
 // rows of neighbours, steps as near to each other as the library takes them
 at::Tensor recurrence_rows(const at::Tensor &t) {
-    return t.stride(1) < (int64_t(1) << 26) ? dense_rows(t) : t.contiguous();
+    return t.stride(1) < (int64_t(1) << 27) / t.element_size() ? dense_rows(t) : t.contiguous();
 }
 
 struct RecurrenceResult {
