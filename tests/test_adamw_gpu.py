@@ -349,6 +349,17 @@ def test_closure_scheduler_version_and_streams():
             assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("bits", [8, 32])
+def test_parameters_without_elements_alone(bits):
+    params = _params(torch.float32, shapes=[(0,), (3, 0)])
+    opt = HipAdamW(params, state_bits=bits)
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    opt.step()
+    assert [int(opt.state[p]["step"]) for p in params] == [1, 1]
+    assert [m.shape for m in opt.moments(params[1])] == [(3, 0), (3, 0)]
+
+
 def test_refusals():
     p = torch.nn.Parameter(torch.zeros(4, 4, device="cuda"))
     for bad in ({"lr": -1.0}, {"lr": math.nan}, {"betas": (1.0, 0.9)}, {"betas": (0.9, -0.1)}, {"eps": -1e-8},

@@ -176,3 +176,15 @@ def test_recurrence_steps_apart_in_bytes(dtype, most):
     for stride, status in ((most - 1, 0), (most, 1)):
         strides = (ctypes.c_int64 * 2)(0, stride)
         assert lib.pesq_recurrence_backward(p, ANY, strides, None, ANY, None, None, None, None, ANY, ANY, None) == status
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_adamw_of_tensors_without_elements(bits):
+    """Nothing to do: no address is needed, as such tensors have none."""
+
+    options = _lib.AdamwOptions(dtype=0, state_bits=bits, step=1, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8)
+    tensors = (_lib.AdamwTensor * 2)()
+    assert _lib.library().pesq_adamw_step(tensors, 2, options, None, None, None, None, None) == 0
+    tensors[1] = _lib.AdamwTensor(param=ANY, grad=ANY, count=1, first=0)
+    assert _lib.library().pesq_adamw_step(tensors, 2, options, None, None, None, None, None) == 1
+    assert "null argument" in _message()

@@ -299,15 +299,14 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                    "betas have to be in [0, 1)");
     const bool eight = o->state_bits == 8;
     const int64_t tile = tile_elements(eight);
-    PESQ_CHECK_ARG(count == 0 || (exp_avg && exp_avg_sq && (!eight || (exp_avg_scale && exp_avg_sq_scale))),
-                   "null argument");
+    const bool arrays = exp_avg && exp_avg_sq && (!eight || (exp_avg_scale && exp_avg_sq_scale));
     for (const void *array : {exp_avg, exp_avg_sq}) {
         PESQ_CHECK_ARG(reinterpret_cast<uintptr_t>(array) % 16 == 0, "the moments start at multiples of 16 bytes");
     }
     for (int64_t k = 0; k < count; ++k) {
         PESQ_CHECK_ARG(tensors[k].count >= 0 && tensors[k].first >= 0 && tensors[k].first % kBlock == 0,
                        "tensor %lld has no place in the moments", (long long)k);
-        PESQ_CHECK_ARG(tensors[k].count == 0 || (tensors[k].param && tensors[k].grad), "null argument");
+        PESQ_CHECK_ARG(tensors[k].count == 0 || (arrays && tensors[k].param && tensors[k].grad), "null argument");
         PESQ_CHECK_ARG(tensors[k].count <= kMostTiles * tile && tensors[k].first < (int64_t(1) << 40),
                        "tensor %lld is too large", (long long)k);
     }

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kMostNormThreads)
     float *out = part + int64_t(blockIdx.x) * 2 * p.channels;
     for (int g = 0; g < at.groups; ++g) {
         if (at.group == g) {
-each_channel<V, E, N>(p, at.lane, [&](int c, int k) {
+            each_channel<V, E, N>(p, at.lane, [&](int c, int k) {
                 float both_c = sum_both[k], next_c = sum_next[k];
                 if (g > 0) {
                     both_c += sums[c];
