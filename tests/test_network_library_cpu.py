@@ -188,3 +188,11 @@ def test_adamw_of_tensors_without_elements(bits):
     tensors[1] = _lib.AdamwTensor(param=ANY, grad=ANY, count=1, first=0)
     assert _lib.library().pesq_adamw_step(tensors, 2, options, None, None, None, None, None) == 1
     assert "null argument" in _message()
+
+
+def test_adamw_moments_fit_a_launch():
+    """Work items of a launch, four elements each in whole workgroups, stay below 2^32."""
+
+    for count, message in ((2**34 - 256, "elements"), (2**34 - 1024, "null argument"), (2**34, "elements")):
+        assert _lib.library().pesq_adamw_moments(None, None, None, None, count, None, None, None) == 1
+        assert message in _message()

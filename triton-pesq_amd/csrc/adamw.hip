@@ -286,10 +286,11 @@ static void launch_adamw(const AdamList &list, int dtype, bool eight, uint32_t t
 
 using namespace pesq;
 
+static constexpr int64_t kMostTiles = (int64_t(1) << 32) / kAdamThreads - 1;  // workgroups of a launch
+
 extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                                const pesq_adamw_options *o, void *exp_avg, void *exp_avg_sq,
                                float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
-    constexpr int64_t kMostTiles = (int64_t(1) << 32) / kAdamThreads - 1;  // of a launch
     PESQ_CHECK_ARG(o != nullptr && count >= 0 && (tensors || count == 0), "null argument");
     PESQ_CHECK_ARG(known_type(o->dtype), "unknown element type %d", int(o->dtype));
     PESQ_CHECK_ARG(o->state_bits == 32 || o->state_bits == 8, "moments have 32 or 8 bits, got %d",
@@ -349,8 +350,8 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
 extern "C" int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq,
                                   const float *exp_avg_scale, const float *exp_avg_sq_scale,
                                   int64_t count, float *m, float *v, hipStream_t stream) {
-    PESQ_CHECK_ARG(count >= 0 && count % kBlock == 0 && count < (int64_t(1) << 34),
-                   "whole blocks of %d elements, 2^34 elements at most, got %lld", kBlock, (long long)count);
+    PESQ_CHECK_ARG(count >= 0 && count % kBlock == 0 && count <= kMostTiles * kAdamThreads * kValues,
+                   "whole blocks of %d elements, 2^34 - 1024 elements at most, got %lld", kBlock, (long long)count);
     if (count == 0) return PESQ_OK;
     PESQ_CHECK_ARG(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && m && v, "null argument");
     for (const void *array : {exp_avg, exp_avg_sq, static_cast<const void *>(m), static_cast<const void *>(v)}) {
