@@ -26,10 +26,9 @@ void with_type(int dtype, Fn fn) {
     }
 }
 
-// 2^x and log2(x) by the hardware's instructions (one unit in the last place,
+// 2^x by the hardware's instruction (one unit in the last place,
 // results below the normal range are flushed), and 1/x likewise
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
 
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -553,7 +553,8 @@ __global__ void __launch_bounds__(kSumShares *kSumColumns)
                             float rate, float *g_decay) {
     const int64_t c = int64_t(blockIdx.x) * kSumColumns + threadIdx.x % kSumColumns;
     const float sum = sum_parts(part, rows, channels, c, channels);
-    if (threadIdx.x < kSumColumns && c < channels) g_decay[c] = sum * (rate * sigmoid_fast(decay[c]));
+    // (the exact sigmoid: its error would be the whole sum's)
+    if (threadIdx.x < kSumColumns && c < channels) g_decay[c] = sum * (rate / (1.0f + expf(-decay[c])));
 }
 
 // kPending into all words, and open_log2 of every channel into rates
