@@ -187,6 +187,34 @@ def test_zero_tiny_and_non_finite_gradients():
             assert torch.isfinite(state["exp_avg_scale"][2:]).all() and torch.isfinite(m[512:]).all()
 
 
+def test_second_moment_beyond_float32():
+    """A finite gradient whose square is infinite, then ordinary ones.  With 8 bits
+    the block's scale is infinite, and its second moments are NaN from the next
+    step on, like 0 times infinity in the plain form: so are its weights, and none
+    takes a finite value from them.  With 32 bits that element alone stands still."""
+
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(600, device="cuda"))
+        opt = HipAdamW([p], lr=1e-3, weight_decay=0.0, state_bits=bits)
+        for step in range(3):
+            p.grad = torch.full((600,), 1e-3, device="cuda")
+            if step == 0:
+                p.grad[5] = 2e19
+            opt.step()
+            if step == 0:
+                assert p[5] == 1 and torch.isfinite(p).all()
+        block = torch.zeros(600, dtype=torch.bool)
+        if bits == 8:
+            block[:256] = True
+            assert torch.isnan(p.detach().cpu()[block]).all()
+            assert torch.isinf(opt.state[p]["exp_avg_sq_scale"][0]) or torch.isnan(opt.state[p]["exp_avg_sq_scale"][0])
+        else:
+            block[5] = True
+            assert p[5] == 1
+        # the others take three full steps of the learning rate
+        assert torch.allclose(p.detach().cpu()[~block], torch.tensor(1 - 3e-3), rtol=1e-5)
+
+
 def test_without_eps():
     """eps = 0: no update where the moments are zero, a full one where the second
     moment is far below what its square can hold in float32."""

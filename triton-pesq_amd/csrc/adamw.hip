@@ -78,7 +78,9 @@ __device__ __forceinline__ float adamw(float p, float g, float &m, float &v, con
     // The hardware's root and reciprocal, each within one unit in the last place.
     // A second moment below 2^-120, where float32 soon has fewer digits and the
     // root flushes them, counts as 2^-120: with eps = 0 there is still a quotient.
-    const float update = m * rcp_fast(__builtin_amdgcn_sqrtf(fmaxf(v, 0x1p-120f)) * a.correction + a.eps);
+    // (a NaN, as all of a block are whose scale is infinite, stays one)
+    const float held = v < 0x1p-120f ? 0x1p-120f : v;
+    const float update = m * rcp_fast(__builtin_amdgcn_sqrtf(held) * a.correction + a.eps);
     return p * a.keep - update * a.step_size;
 }
 
