@@ -203,6 +203,48 @@ def test_resets_drop_whatever_the_state_holds():
             assert torch.equal(grads[name][1], clean[2][name][1]), name
 
 
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("resets", [False, True])
+def test_states_that_are_not_finite_stay_so(resets, reverse):
+    """Over thousands of steps without a reset, whose factors' product is 0 in
+    float32 (0.9^1024 is 1e-47), in both passes; and up to the reset where there is one."""
+
+    def at(n):  # step n of the fold
+        return time - 1 - n if reverse else n
+
+    time = 4000
+    t = _inputs(2, time, 66, torch.float32, seed=10)
+    t["recur"].fill_(20.0)
+    t["decay"].fill_(math.log(math.expm1(-math.log(0.9) / 8.0)))
+    if resets:
+        t["reset"] = torch.zeros(2, time, dtype=torch.bool)
+        t["reset"][0, at(3000)] = True
+    for bad in (math.nan, math.inf, -math.inf):
+        t["initial"][0, :33] = bad
+        t["x"][1, at(10), 33:] = bad
+        y, last, _ = _run(t, reverse)
+        y = y.flip(1) if reverse else y
+        end = 3000 if resets else time
+        assert not torch.isfinite(y[0, :end, :33]).any()
+        assert not torch.isfinite(y[1, 10:, 33:]).any() and not torch.isfinite(last[1, 33:]).any()
+        assert torch.isfinite(y[0, end:]).all() and torch.isfinite(last[0, :33]).all() == resets
+        assert torch.isfinite(y[0, :, 33:]).all() and torch.isfinite(y[1, :10]).all() and torch.isfinite(y[1, :, :33]).all()
+
+    # the gradient's carry, towards earlier steps
+    t = dict(t, x=torch.randn(2, time, 66), initial=torch.randn(2, 66))
+    t["g_last"][0, :33] = math.nan
+    t["g_y"][1, at(3500), 33:] = math.inf
+    _, _, grads = _run(t, reverse)
+    g = grads["x"].flip(1) if reverse else grads["x"]
+    assert not torch.isfinite(g[0, end if resets else 0:, :33]).any()
+    assert not torch.isfinite(g[1, :3501, 33:]).any()
+    assert not torch.isfinite(grads["initial"][1, 33:]).any()
+    assert torch.isfinite(grads["initial"][0, :33]).all() == resets
+    if resets:
+        assert torch.isfinite(g[0, :end, :33]).all()
+    assert torch.isfinite(g[1, 3501:]).all() and torch.isfinite(g[:, :, 33:][0]).all()
+
+
 def test_every_step_reset_and_empty_sizes():
     t = _inputs(2, 35, 64, torch.float32, seed=11)
     t["reset"] = torch.ones(2, 35, dtype=torch.bool)

@@ -172,13 +172,26 @@ __device__ __forceinline__ void store_channel(Buffer buffer, uint32_t channel, i
     }
 }
 
-// The map h -> a h + b of a stretch of steps.  a is 0 where a reset (or a decay
-// beyond float32) drops what came before, whatever it is.
+// The map h -> a h + b of a stretch of steps.  a is -0 where a reset drops what
+// came before, whatever it is.  Any other a is +0 at least, a product that became
+// 0 over many steps too: a NaN or an infinite h is not finite after it either, as
+// step by step.
 struct Pair {
     float a, b;
-    __device__ __forceinline__ float operator()(float h) const { return a == 0.0f ? b : fmaf(a, h, b); }
+    // kReset: whether there are resets at all
+    template <bool kReset>
+    __device__ __forceinline__ bool drops() const {
+        return kReset && __float_as_uint(a) == 0x80000000u;
+    }
+    template <bool kReset>
+    __device__ __forceinline__ float after(float h) const {
+        return drops<kReset>() ? b : fmaf(a, h, b);
+    }
     // this one, then `next`
-    __device__ __forceinline__ Pair then(const Pair &next) const { return {a * next.a, next(b)}; }
+    template <bool kReset>
+    __device__ __forceinline__ Pair then(const Pair &next) const {
+        return {next.drops<kReset>() ? next.a : a * next.a, next.after<kReset>(b)};
+    }
 };
 
 __device__ __forceinline__ void publish(uint64_t *word, Pair p) {
@@ -283,7 +296,7 @@ struct Early {
 // of the chunks before it; publishes this chunk's pair, and for the last of kFan
 // chunks that of all of them.  The parts' pairs are in LDS; the wavefronts wait
 // for some words each, and the first one folds them.
-template <bool kBack>
+template <bool kBack, bool kReset>
 __device__ __forceinline__ float join_chunks(const RecArgs &p, const Place &at, const Published &of,
                                              const Early &early, int lane, int wave, int waves, float initial,
                                              Shared &lds) {
@@ -291,7 +304,7 @@ __device__ __forceinline__ float join_chunks(const RecArgs &p, const Place &at, 
     Pair own{1.0f, 0.0f}, near{1.0f, 0.0f};
     float h = initial;
     if (wave == 0) {
-        for (int w = 0; w < waves; ++w) own = own.then(lds.parts[kBack ? waves - 1 - w : w][lane]);
+        for (int w = 0; w < waves; ++w) own = own.then<kReset>(lds.parts[kBack ? waves - 1 - w : w][lane]);
         publish(of.pairs + at.chunk * of.stride, own);
     }
     for (int64_t first = 0; first < of.items;) {
@@ -310,17 +323,17 @@ __device__ __forceinline__ float join_chunks(const RecArgs &p, const Place &at, 
             for (int k = 0; k < here; ++k) {
                 const Pair q = lds.words[k][lane];
                 if (first + k < of.in_fan) {
-                    near = near.then(q);
+                    near = near.then<kReset>(q);
                 } else {
-                    h = q(h);
+                    h = q.after<kReset>(h);
                 }
             }
-            if (first == 0 && of.in_fan == kFan - 1) publish(of.joined + of.fan * of.stride, near.then(own));
+            if (first == 0 && of.in_fan == kFan - 1) publish(of.joined + of.fan * of.stride, near.then<kReset>(own));
         }
         first += here;
         if (first < of.items) __syncthreads();
     }
-    if (wave == 0) lds.heads[lane] = near(h);
+    if (wave == 0) lds.heads[lane] = near.after<kReset>(h);
     __syncthreads();
     return lds.heads[lane];
 }
@@ -435,14 +448,14 @@ __global__ void __launch_bounds__(kMaxWaves *kWave, 5)
             const Gates g = gates(static_cast<float>(part.e[0][s]), static_cast<float>(part.e[1][s]), k);
             a[s] = there ? g.a : 1.0f;
             in[s] = there ? g.s * g.open_i * static_cast<float>(part.e[2][s]) : 0.0f;
-            own.a = drop ? 0.0f : own.a * a[s];
+            own.a = drop ? -0.0f : own.a * a[s];
             own.b = drop ? in[s] : fmaf(a[s], own.b, in[s]);
         }
     });
     lds.parts[wave][lane] = own;
     __syncthreads();
-    float h = join_chunks<false>(p, at, of, early, lane, wave, waves, part.initial, lds);
-    for (int w = 0; w < wave; ++w) h = lds.parts[w][lane](h);
+    float h = join_chunks<false, kReset>(p, at, of, early, lane, wave, waves, part.initial, lds);
+    for (int w = 0; w < wave; ++w) h = lds.parts[w][lane].after<kReset>(h);
     if (left > 0) {
         const float *out = starts + (at.b * cdiv(p.time, kSteps) + n0 / kSteps) * p.channels + at.c0;
         store_channel<float>(buffer_of(out, starts), at.channel, 0, h);
@@ -494,14 +507,14 @@ __global__ void __launch_bounds__(kMaxWaves *kWave)
             a[s] = exp2_fast(k * open_r[s]);
             g[s] = there ? static_cast<float>(part.e[3][s]) : 0.0f;
             const float on = there ? a[s] : 1.0f;
-            own.a = drop ? 0.0f : own.a * on;
+            own.a = drop ? -0.0f : own.a * on;
             own.b = drop ? 0.0f : on * (g[s] + own.b);
         }
     });
     lds.parts[wave][lane] = own;
     __syncthreads();
-    float c = join_chunks<true>(p, at, of, early, lane, wave, waves, part.initial, lds), sum = 0.0f;
-    for (int w = waves - 1; w > wave; --w) c = lds.parts[w][lane](c);
+    float c = join_chunks<true, kReset>(p, at, of, early, lane, wave, waves, part.initial, lds), sum = 0.0f;
+    for (int w = waves - 1; w > wave; --w) c = lds.parts[w][lane].after<kReset>(c);
     for_part(left, [&](auto full) {
 #pragma unroll
         for (int s = kSteps - 1; s >= 0; --s) {
