@@ -348,6 +348,32 @@ def test_only_the_gradients_that_are_asked_for():
         g.sum().backward()
 
 
+def test_gradients_of_gradients_are_refused_whatever_the_upstream():
+    """A penalty on a gradient next to another loss: refused where the gradient is a
+    function of an input that wants one, also under a constant upstream; where it is
+    not (y is linear in x and the initial state), its second derivative is 0."""
+
+    t = _inputs(2, 20, 33, torch.float32, seed=25)
+    #            of a gradient of                          by the inputs
+    depends = {"x": {"recur", "input", "decay"}, "recur": set(NAMES), "input": {"x", "recur", "input", "decay"},
+               "decay": set(NAMES), "initial": {"recur", "decay"}}
+    for of in NAMES:
+        for by in NAMES:
+            d = {k: t[k].cuda() for k in NAMES}
+            for name in (of, by):
+                d[name].requires_grad_()
+            y, last = gated_recurrence(*(d[k] for k in NAMES[:4]), initial_state=d["initial"])
+            (g,) = torch.autograd.grad(y.sum() + last.sum(), d[of], create_graph=True)
+            loss = g.square().sum() + sum(v.square().sum() for v in d.values())
+            # (with `of` = `by` alone, what matters is whether the gradient depends on itself)
+            if depends[of] & {of, by}:
+                with pytest.raises(RuntimeError, match="once_differentiable"):
+                    loss.backward()
+            else:
+                loss.backward()
+                assert torch.equal(d[by].grad, 2 * d[by].detach()), (of, by)
+
+
 def test_refusals():
     t = {k: v.cuda() for k, v in _inputs(2, 8, 16, torch.float32).items() if v is not None}
     x, recur, gate, decay = t["x"], t["recur"], t["input"], t["decay"]

@@ -279,6 +279,42 @@ def test_only_the_gradients_that_are_asked_for():
         g.sum().backward()
 
 
+def test_gradients_of_gradients_are_refused_whatever_the_upstream():
+    """A penalty on a gradient next to another loss: refused where the gradient is a
+    function of an input that wants one, also under a constant upstream; where it is
+    not (x_out is linear in x, the weight and the scale), its second derivative is 0."""
+
+    t, _ = _inputs((9, 130), torch.float32, torch.float32, seed=16)
+    everything = set(NAMES)
+    #                    of a gradient of                   by the inputs
+    depends = {"x_out": {"x": set(), "branch": {"branch", "gate", "weight", "scale"},
+                         "gate": {"branch", "gate", "weight", "scale"}, "weight": {"branch", "gate", "scale"},
+                         "scale": {"branch", "gate", "weight"}, "next_weight": set()},
+               "n": {**{k: everything for k in NAMES[:5]}, "next_weight": everything - {"next_weight"}}}
+    for which, output in enumerate(depends):
+        for of in NAMES:
+            for by in NAMES:
+                if output == "x_out" and of == "next_weight":
+                    continue  # not connected
+                d = {k: v.cuda() for k, v in t.items()}
+                for name in (of, by):
+                    d[name].requires_grad_()
+                out = residual_norm(d["x"], d["branch"], d["weight"], gate=d["gate"], scale=d["scale"],
+                                    next_weight=d["next_weight"])[which]
+                (g,) = torch.autograd.grad(out.sum(), d[of], create_graph=True)
+                loss = g.square().sum() + sum(v.square().sum() for v in d.values())
+                if depends[output][of] & {of, by}:
+                    with pytest.raises(RuntimeError, match="once_differentiable"):
+                        loss.backward()
+                else:
+                    loss.backward()
+                    assert torch.equal(d[by].grad, 2 * d[by].detach()), (output, of, by)
+    x, w = t["x"].cuda().requires_grad_(), t["weight"].cuda()
+    (g,) = torch.autograd.grad(pre_norm(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (x.sum() + g.square().sum()).backward()
+
+
 def test_no_rows():
     t, up = _inputs((0, 40), torch.float32, torch.float32)
     got = _run(t, up)

@@ -39,13 +39,30 @@ at::Tensor of_type(const at::Tensor &t, at::ScalarType type) {
     return t.scalar_type() == type ? t : t.to(type);
 }
 
-// the gradients, with a derivative that raises where a double backward would need one
-void mark_once(variable_list &grads, const variable_list &upstream) {
+// a bit for each input that requires a gradient, asked for in this backward or not
+template <size_t N>
+int64_t requiring(const std::array<const at::Tensor *, N> &inputs) {
+    int64_t bits = 0;
+    for (size_t k = 0; k < N; ++k) {
+        if (inputs[k]->defined() && inputs[k]->requires_grad()) bits |= int64_t(1) << k;
+    }
+    return bits;
+}
+
+// The gradients, with a derivative that raises where a double backward would need
+// one: where an upstream gradient wants it, or an input of `requiring` that the
+// gradient is a function of, by `depends` (of each gradient, in the same bits).
+template <size_t N>
+void mark_once(variable_list &grads, const variable_list &upstream, int64_t requiring,
+               const std::array<int64_t, N> &depends) {
+    if (!torch::autograd::GradMode::is_enabled()) return;
     bool needed = false;
     for (const at::Tensor &g : upstream) needed = needed || (g.defined() && g.requires_grad());
-    if (!needed || !torch::autograd::GradMode::is_enabled()) return;
-    for (at::Tensor &g : grads) {
-        if (g.defined()) g = OnceDifferentiable::apply(g.detach().requires_grad_(true));
+    for (size_t k = 0; k < N; ++k) {
+        at::Tensor &g = grads[k];
+        if (g.defined() && (needed || (requiring & depends[k]))) {
+            g = OnceDifferentiable::apply(g.detach().requires_grad_(true));
+        }
     }
 }
 
@@ -154,6 +171,8 @@ struct Recurrence : public torch::autograd::Function<Recurrence> {
         ctx->save_for_backward({r.in.x, r.in.recur, r.in.input, r.in.decay, r.in.initial, r.in.reset, r.starts});
         ctx->saved_data["reverse"] = reverse;
         ctx->saved_data["rate"] = rate;
+        const at::Tensor none;
+        ctx->saved_data["requiring"] = requiring<5>({&x, &recur, &input, &decay, initial ? &*initial : &none});
         return {r.y, r.last};
     }
 
@@ -188,7 +207,12 @@ struct Recurrence : public torch::autograd::Function<Recurrence> {
                                        data(out[1]), data(out[2]), data_or_null<float>(out[3]),
                                        data_or_null<float>(out[4]), data(ws), current_stream(x)),
               "pesq_recurrence_backward");
-        mark_once(out, grads);
+        // G is a function of the factors a, so of the recurrence's gate and the decay;
+        // x and the initial state, in which y is linear, are in the gates' alone
+        constexpr int64_t kX = 1, kRecur = 2, kInput = 4, kDecay = 8, kInitial = 16;
+        constexpr int64_t kFactors = kRecur | kDecay, kAll = kX | kInput | kInitial | kFactors;
+        mark_once<5>(out, grads, ctx->saved_data["requiring"].toInt(),
+                     {kFactors | kInput, kAll, kFactors | kInput | kX, kAll, kFactors});
         return out;
     }
 };
@@ -312,6 +336,10 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
         ctx->set_materialize_grads(false);
         ctx->save_for_backward({r.in.x, r.in.branch, r.in.gate, r.in.post, r.in.scale, r.in.next, r.inverse});
         ctx->saved_data["eps"] = eps;
+        const at::Tensor none;
+        const auto operand = [&](const OptTensor &t) { return t ? &*t : &none; };
+        ctx->saved_data["requiring"] =
+            requiring<6>({&x, operand(branch), operand(gate), operand(post), operand(scale), operand(next)});
         ctx->saved_data["dtype"] = static_cast<int64_t>(r.dtype);
         ctx->saved_data["sizes"] = x.sizes().vec();
         return r.out;
@@ -364,7 +392,13 @@ struct ResidualNorm : public torch::autograd::Function<ResidualNorm> {
                   data_or_null<float>(out[4]), data_or_null<float>(g_next), data(ws),
                   current_stream(in.x)),
               "pesq_residual_norm_backward");
-        mark_once(out, grads);
+        // x' alone is linear in x, the scale and the weight
+        constexpr int64_t kX = 1, kBranch = 2, kGate = 4, kPost = 8, kScale = 16, kNext = 32;
+        constexpr int64_t kOfY = kBranch | kGate, kAll = kX | kOfY | kPost | kScale | kNext;
+        const int64_t of_n = g_n_out.defined() ? kAll : 0;
+        mark_once<6>(out, grads, ctx->saved_data["requiring"].toInt(),
+                     {of_n, of_n | kOfY | kPost | kScale, of_n | kOfY | kPost | kScale, of_n | kOfY | kScale,
+                      of_n | kOfY | kPost, of_n & ~kNext});
         return out;
     }
 };
