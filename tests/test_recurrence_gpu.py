@@ -289,6 +289,30 @@ def test_sequence_in_pieces_and_frame_by_frame():
         _close(state, want[1], _tolerance(torch.float32, 50), "state")
 
 
+def test_a_step_marks_its_state_as_changed():
+    """What has saved the state for its backward raises there, as after torch's own
+    updates in place; a state that requires a gradient is refused."""
+
+    t = {k: v.cuda() for k, v in _inputs(2, 8, 16, torch.float32, seed=14).items() if v is not None}
+    x, recur, gate, decay = t["x"].requires_grad_(), t["recur"], t["input"], t["decay"]
+    frame = x[:, 0].detach(), recur[:, 0], gate[:, 0], decay
+    _, last = gated_recurrence(x, recur, gate, decay)
+    loss = last.square().sum()
+    with pytest.raises(RuntimeError, match="require a gradient"):
+        gated_recurrence_step(*frame, last)
+    with pytest.raises(RuntimeError, match="require a gradient"):
+        gated_recurrence_step(*frame, torch.zeros(2, 16, device="cuda", requires_grad=True))
+    torch.autograd.grad(loss, x, retain_graph=True)
+    gated_recurrence_step(*frame, last.detach())
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, x)
+    with torch.inference_mode():
+        state = torch.zeros(2, 16, device="cuda")
+        assert torch.isfinite(gated_recurrence_step(*frame, state)).all() and (state != 0).any()
+    with torch.no_grad():
+        gated_recurrence_step(*frame, torch.zeros(2, 16, device="cuda", requires_grad=True))
+
+
 def test_gradient_against_differences():
     """The directional derivative of a weighted sum of the outputs, against its
     central difference: the step's cube (1e-2) and float32 results set 2e-3."""

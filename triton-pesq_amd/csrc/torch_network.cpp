@@ -66,6 +66,11 @@ void mark_once(variable_list &grads, const variable_list &upstream, int64_t requ
     }
 }
 
+// t was updated in place: a node that has saved it raises in its backward
+void written(const at::Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void *data(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // ---------------------------------------------------------------------------
@@ -246,6 +251,8 @@ at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
     check_recurrence_inputs(x, recur, input, decay, 2, "[batch, channels]");
     check_state(state, "state", x);
     TORCH_CHECK(state.is_contiguous(), "`state` is updated in place and has to be contiguous");
+    TORCH_CHECK(!(state.requires_grad() && torch::autograd::GradMode::is_enabled()),
+                "`state` is updated in place and cannot require a gradient");
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard no_grad;
     const RecurrenceInputs in{dense_rows(x), dense_rows(recur), dense_rows(input),
@@ -254,6 +261,7 @@ at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
     at::Tensor y = at::empty(x.sizes(), x.options());
     check(pesq_recurrence_step(&p, state.data_ptr<float>(), y.data_ptr(), current_stream(x)),
           "pesq_recurrence_step");
+    written(state);
     return y;
 }
 
@@ -564,7 +572,7 @@ class AdamWPlan {
         for (size_t k = 0; k < params.size(); ++k) {
             if (!params[k].grad().defined()) continue;
             ++steps[k];
-            if (!params[k].is_inference()) params[k].unsafeGetTensorImpl()->bump_version();
+            written(params[k]);
         }
     }
 

@@ -42,7 +42,8 @@ def gated_recurrence(x, recur_gate, input_gate, decay, *, initial_state=None, re
 
 def gated_recurrence_step(x, recur_gate, input_gate, decay, state, *, rate=8.0):
     """``y`` ``[batch, channels]`` of one frame; ``state`` (float32, as
-    ``gated_recurrence`` returns it) is updated in place.  No gradient."""
+    ``gated_recurrence`` returns it) is updated in place, and cannot require a
+    gradient while these are recorded.  No gradient."""
 
     return _lib.torch_ext().gated_recurrence_step(x, recur_gate, input_gate, decay, state, float(rate))
 
