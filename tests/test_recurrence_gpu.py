@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from torch_pesq.hip_ops.recurrence import HipGatedRecurrence, gated_recurrence, gated_recurrence_step
 
@@ -396,6 +397,27 @@ def test_gradients_of_gradients_are_refused_whatever_the_upstream():
             else:
                 loss.backward()
                 assert torch.equal(d[by].grad, 2 * d[by].detach()), (of, by)
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any input raises, whether gradients are recorded or not."""
+
+    t = {k: v.cuda() for k, v in _inputs(2, 8, 16, torch.float32, seed=26).items() if v is not None}
+    t["state"] = torch.zeros(2, 16, device="cuda")
+    with forward_ad.dual_level():
+        for name in (*NAMES, "state"):
+            d = dict(t, **{name: forward_ad.make_dual(t[name], torch.ones_like(t[name]))})
+            for recorded in (True, False):
+                with torch.set_grad_enabled(recorded), pytest.raises(RuntimeError, match="jvp"):
+                    if name == "state":
+                        gated_recurrence_step(*(d[k][:, 0] for k in NAMES[:3]), d["decay"], d["state"])
+                    else:
+                        gated_recurrence(*(d[k] for k in NAMES[:4]), initial_state=d["initial"])
+        # in a level, but without a tangent
+        gated_recurrence(*(t[k] for k in NAMES[:4]))
+    x = t["x"].requires_grad_()
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="jvp"):
+        gated_recurrence(forward_ad.make_dual(x, torch.ones_like(x)), *(t[k] for k in NAMES[1:4]))
 
 
 def test_refusals():

@@ -12,6 +12,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from torch_pesq.hip_ops.norm import pre_norm, residual_norm
 
@@ -313,6 +314,26 @@ def test_gradients_of_gradients_are_refused_whatever_the_upstream():
     (g,) = torch.autograd.grad(pre_norm(x, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         (x.sum() + g.square().sum()).backward()
+
+
+def test_forward_mode_is_refused():
+    """A tangent on any input raises, whether gradients are recorded or not; weights
+    that are converted first among them."""
+
+    t, _ = _inputs((4, 32), torch.float32, torch.float32, seed=17)
+    t = {k: v.cuda() for k, v in t.items()}
+    t["weight"] = t["weight"].half()
+    with forward_ad.dual_level():
+        for name in NAMES:
+            d = dict(t, **{name: forward_ad.make_dual(t[name], torch.ones_like(t[name]))})
+            for recorded in (True, False):
+                with torch.set_grad_enabled(recorded), pytest.raises(RuntimeError, match="jvp"):
+                    residual_norm(d["x"], d["branch"], d["weight"], gate=d["gate"], scale=d["scale"],
+                                  next_weight=d["next_weight"])
+        with pytest.raises(RuntimeError, match="jvp"):
+            pre_norm(forward_ad.make_dual(t["x"], torch.ones_like(t["x"])), t["weight"])
+        # in a level, but without a tangent
+        residual_norm(t["x"], t["branch"], t["weight"])
 
 
 def test_no_rows():

@@ -8,6 +8,7 @@
 
 #include <array>
 #include <optional>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -69,6 +70,25 @@ void mark_once(variable_list &grads, const variable_list &upstream, int64_t requ
 // t was updated in place: a node that has saved it raises in its backward
 void written(const at::Tensor &t) {
     if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// Calls that need no node are spared it, and with it the node's refusal of forward
+// mode derivatives, which the kernels do not have
+void check_no_tangent(const at::Tensor &t) {
+    TORCH_CHECK(!t.unsafeGetTensorImpl()->_fw_grad(0, t).defined(),
+                "forward mode derivatives (jvp) are not implemented for this operator");
+}
+
+template <class... Tensors>
+void check_no_tangents(const Tensors &...tensors) {
+    const auto one = [](const auto &t) {
+        if constexpr (std::is_same_v<std::decay_t<decltype(t)>, OptTensor>) {
+            if (t) check_no_tangent(*t);
+        } else {
+            check_no_tangent(t);
+        }
+    };
+    (one(tensors), ...);
 }
 
 void *data(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
@@ -239,7 +259,7 @@ std::vector<at::Tensor> gated_recurrence(const at::Tensor &x, const at::Tensor &
                       (x.requires_grad() || recur.requires_grad() || input.requires_grad() ||
                        decay.requires_grad() || (initial && initial->requires_grad()));
     if (keep) return Recurrence::apply(x, recur, input, decay, initial, reset, reverse, rate);
-    // (a call without a gradient is spared the node)
+    check_no_tangents(x, recur, input, decay, initial);
     const at::NoGradGuard no_grad;
     const RecurrenceResult r = run_recurrence(x, recur, input, decay, initial, reset, reverse, rate, false);
     return {r.y, r.last};
@@ -253,6 +273,7 @@ at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
     TORCH_CHECK(state.is_contiguous(), "`state` is updated in place and has to be contiguous");
     TORCH_CHECK(!(state.requires_grad() && torch::autograd::GradMode::is_enabled()),
                 "`state` is updated in place and cannot require a gradient");
+    check_no_tangents(x, recur, input, decay, state);
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard no_grad;
     const RecurrenceInputs in{dense_rows(x), dense_rows(recur), dense_rows(input),
@@ -458,6 +479,7 @@ std::vector<at::Tensor> residual_norm(const at::Tensor &x, const OptTensor &bran
     if (keep && torch::autograd::GradMode::is_enabled()) {
         return ResidualNorm::apply(x, branch, gate, w, s, n, code, eps);
     }
+    check_no_tangents(x, branch, gate, w, s, n);
     const at::NoGradGuard no_grad;
     return run_norm(x, branch, gate, w, s, n, code, eps, false).out;
 }
