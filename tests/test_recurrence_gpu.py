@@ -399,6 +399,28 @@ def test_gradients_of_gradients_are_refused_whatever_the_upstream():
                 assert torch.equal(d[by].grad, 2 * d[by].detach()), (of, by)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float64])
+def test_decays_of_other_types(dtype):
+    """A module converted as a whole: the decay's value in float32, and its gradient
+    rounded to its own type."""
+
+    module = HipGatedRecurrence(48).cuda().to(dtype)
+    assert module.decay.dtype == dtype
+    t = _inputs(2, 40, 48, torch.bfloat16 if dtype == torch.float64 else dtype, seed=27)
+    t["decay"] = module.decay.detach().float().cpu()
+    want = _run(t)
+    frames = [t[k].cuda() for k in ("x", "recur", "input")]
+    y, last = module(*frames, initial_state=t["initial"].cuda())
+    assert torch.equal(y, want[0]) and torch.equal(last, want[1])
+    (g,) = torch.autograd.grad((y, last), module.decay, (t["g_y"].cuda(), t["g_last"].cuda()))
+    assert g.dtype == dtype and torch.equal(g, want[2]["decay"].to(dtype))
+    state = t["initial"].cuda()
+    out = module.step(*(v[:, 0] for v in frames), state)
+    assert torch.equal(out, gated_recurrence_step(*(v[:, 0] for v in frames), t["decay"].cuda(), t["initial"].cuda()))
+    with pytest.raises(RuntimeError, match="decay"):
+        gated_recurrence(*frames, torch.zeros(48, dtype=torch.int32, device="cuda"))
+
+
 def test_forward_mode_is_refused():
     """A tangent on any input raises, whether gradients are recorded or not."""
 

@@ -140,8 +140,8 @@ void check_recurrence_inputs(const at::Tensor &x, const at::Tensor &recur, const
                     x.scalar_type(), ", got ", t->scalar_type());
     }
     check_gpu(decay, "decay", x);
-    TORCH_CHECK(decay.scalar_type() == at::kFloat && decay.dim() == 1 && decay.size(0) == x.size(-1),
-                "`decay` has to be float32 [channels], got ", decay.scalar_type(), " ", decay.sizes());
+    TORCH_CHECK(decay.is_floating_point() && decay.dim() == 1 && decay.size(0) == x.size(-1),
+                "`decay` has to be a floating [channels] tensor, got ", decay.scalar_type(), " ", decay.sizes());
 }
 
 void check_state(const at::Tensor &state, const char *name, const at::Tensor &x) {
@@ -243,10 +243,11 @@ struct Recurrence : public torch::autograd::Function<Recurrence> {
 };
 
 std::vector<at::Tensor> gated_recurrence(const at::Tensor &x, const at::Tensor &recur,
-                                         const at::Tensor &input, const at::Tensor &decay,
+                                         const at::Tensor &input, const at::Tensor &any_decay,
                                          const OptTensor &initial, const OptTensor &reset,
                                          bool reverse, double rate) {
-    check_recurrence_inputs(x, recur, input, decay, 3, "[batch, time, channels]");
+    check_recurrence_inputs(x, recur, input, any_decay, 3, "[batch, time, channels]");
+    const at::Tensor decay = of_type(any_decay, at::kFloat);
     if (initial) check_state(*initial, "initial_state", x);
     if (reset) {
         check_gpu(*reset, "reset", x);
@@ -277,7 +278,7 @@ at::Tensor gated_recurrence_step(const at::Tensor &x, const at::Tensor &recur,
     const c10::DeviceGuard guard(x.device());
     const at::NoGradGuard no_grad;
     const RecurrenceInputs in{dense_rows(x), dense_rows(recur), dense_rows(input),
-                              decay.contiguous(), {}, {}};
+                              of_type(decay, at::kFloat).contiguous(), {}, {}};
     const pesq_recurrence p = in.call(false, rate);
     at::Tensor y = at::empty(x.sizes(), x.options());
     check(pesq_recurrence_step(&p, state.data_ptr<float>(), y.data_ptr(), current_stream(x)),

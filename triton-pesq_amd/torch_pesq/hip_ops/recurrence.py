@@ -27,8 +27,8 @@ def gated_recurrence(x, recur_gate, input_gate, decay, *, initial_state=None, re
 
     ``x`` and the gates' arguments share one type (float32, bfloat16 or float16)
     and may be strided views, such as the parts of one linear layer's output;
-    ``decay`` is float32 ``[channels]``, ``initial_state`` float32 ``[batch,
-    channels]`` (zero if ``None``).  Where ``reset`` (bool ``[batch, time]``) is
+    ``decay`` is floating ``[channels]`` (converted where it is not float32),
+    ``initial_state`` float32 ``[batch, channels]`` (zero if ``None``).  Where ``reset`` (bool ``[batch, time]``) is
     true the state before that step is dropped, whatever it holds: the start of
     another utterance in the same row.  ``reverse`` runs from the last step to
     the first; the last state is then the one after step 0.  Differentiable once
