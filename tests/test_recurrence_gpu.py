@@ -181,6 +181,36 @@ def test_closed_and_open_gates():
         _close(got[2][name], want[2][name], _tolerance(torch.float32, 50), name)
 
 
+def test_decays_without_end():
+    """Infinite decays and those near float32's ends: forgotten at once (a = 0) or
+    kept for good (a = 1), a shut gate keeps either way; NaN stays in its channel."""
+
+    for steps in (40, 200):
+        t = _inputs(2, steps, 64, torch.float32, seed=28)
+        t["recur"][:, 5:9] = -200.0
+        t["recur"][:, 9] = -math.inf
+        finite = dict(t, decay=torch.full((64,), 1e4))
+        finite["decay"][32:] = -1e4
+        want = _run(finite)
+        _close(want[0], _reference(finite, grads=False)[0], _tolerance(torch.float32, steps), "y")
+        for most in (math.inf, 3e38, 2.3e38, 1e20):
+            t["decay"][:32], t["decay"][32:] = most, -most
+            got = _run(t)
+            # a, s and their slopes are the same for all of these
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), most
+            for name in ("x", "input", "initial"):
+                assert torch.equal(got[2][name], want[2][name]), (most, name)
+            assert (got[2]["recur"] == 0).all() and torch.isfinite(got[2]["decay"]).all(), most
+        t["decay"][3] = math.nan
+        got = _run(t)
+        others = torch.arange(64) != 3
+        assert torch.isnan(got[0][..., 3]).all() and torch.equal(got[0][..., others], want[0][..., others])
+    frame = [t[k][:, 5].cuda() for k in ("x", "recur", "input")]
+    state = t["initial"].cuda()
+    gated_recurrence_step(*frame, t["decay"].cuda(), state)
+    assert torch.isnan(state[:, 3]).all() and torch.equal(state[:, others], t["initial"].cuda()[:, others])
+
+
 def test_resets_drop_whatever_the_state_holds():
     """NaN and infinities before a reset, in the initial state too, do not reach
     the steps after it, nor the gradients of what comes after."""

@@ -39,6 +39,7 @@
 // The backward does the same towards earlier steps for G, and takes the states
 // themselves from those that the forward keeps, in float32, before each part:
 // they are neither stored step by step nor rounded.
+#include <cfloat>
 #include <cmath>
 #include <type_traits>
 
@@ -76,10 +77,11 @@ struct RecArgs {
 // the last bits, since its error acts on every step:
 // softplus(d) = max(d, 0) + log(1 + y), y = exp(-|d|).  The exponential's argument
 // is carried in two parts; log(1 + y) = 2 artanh(z), z = y / (2 + y) <= 1/3, by
-// its series up to z^15.
+// its series up to z^15.  Finite for every decay but NaN, which stays one: a gate
+// that is shut (sigmoid 0) keeps the state whatever the decay.
 __device__ __forceinline__ float open_log2(float decay, float rate) {
     constexpr float kLog2eRest = 1.92596299e-8f;  // log2(e) = kLog2e + this
-    const float d = fabsf(decay), x = kLog2e * d;
+    const float d = fminf(fabsf(decay), 128.0f), x = kLog2e * d;  // (y is 0 from 104 on)
     const float rest = fmaf(kLog2e, d, -x) + kLog2eRest * d;
     float y = exp2_fast(-x);
     y = fmaf(-kLn2 * rest, y, y);
@@ -95,8 +97,8 @@ __device__ __forceinline__ float open_log2(float decay, float rate) {
     p = fmaf(p, t, 1.0f / 5.0f);
     p = fmaf(p, t, 1.0f / 3.0f);
     p = fmaf(p * t, z, z);
-    const float softplus = fmaf(2.0f, p, fmaxf(decay, 0.0f));
-    return -softplus * (rate * kLog2e);
+    const float softplus = fmaf(2.0f, p, decay < 0.0f ? 0.0f : decay), k = -softplus * (rate * kLog2e);
+    return k < -FLT_MAX ? -FLT_MAX : k;
 }
 
 // -expm1(-w) / w on [0, 0.5]: the polynomial of least largest relative error
