@@ -526,7 +526,7 @@ typedef struct pesq_recurrence {
     int64_t batch, time, channels;
     int32_t dtype; /* of x, the gates, y and their gradients */
     int32_t reverse;
-    double rate; /* > 0 */
+    double rate; /* > 0, at most 2^126; held in float32 */
     const void *x, *recur_gate, *input_gate;
     int64_t strides[3][2];
     const float *decay;

@@ -41,6 +41,20 @@ def test_recurrence_refuses(changes, message):
         assert re.search(message, _message())
 
 
+@pytest.mark.parametrize("rate,status", [(2.0**126, 0), (1e-30, 0), (2.0**127, 1), (1e39, 1)])
+def test_recurrence_rates_fit_float32(rate, status):
+    """The kernels hold the rate times log2(e) in float32, where 1e39 would be infinite
+    and the product with a softplus of 0 a NaN."""
+
+    assert _lib.library().pesq_recurrence_workspace(_recurrence(rate=rate), None, None, None) == status
+    assert status == 0 or "rate" in _message()
+    if status:
+        with pytest.raises(ValueError, match="rate"):
+            HipGatedRecurrence(4, rate=rate)
+    else:
+        HipGatedRecurrence(4, rate=rate)
+
+
 def test_recurrence_null_arguments_and_strides():
     lib = _lib.library()
     for name in ("x", "recur_gate", "input_gate", "decay"):

@@ -614,7 +614,8 @@ static int check_recurrence(const pesq_recurrence *p) {
     PESQ_CHECK_ARG(p->channels <= (int64_t(1) << 24) && p->time <= (int64_t(1) << 32),
                    "a recurrence has at most 2^24 channels and 2^32 steps, got %lld and %lld",
                    (long long)p->channels, (long long)p->time);
-    PESQ_CHECK_ARG(p->rate > 0.0 && std::isfinite(p->rate), "the rate has to be positive and finite");
+    PESQ_CHECK_ARG(p->rate > 0.0 && p->rate <= 0x1p126,  // (float32, times log2(e))
+                   "the rate has to be positive and at most 2^126, got %g", p->rate);
     for (int k = 0; k < 6; ++k) {
         PESQ_CHECK_ARG(p->strides[k / 2][k % 2] >= 0, "negative stride");
         PESQ_CHECK_ARG(k % 2 == 0 || near_steps(p->strides[k / 2][1], p->dtype),

@@ -12,8 +12,6 @@ frame::
 whatever the type of ``x``.  No counterpart in the reference.
 """
 
-import math
-
 import torch
 
 from .. import _lib
@@ -56,8 +54,8 @@ class HipGatedRecurrence(torch.nn.Module):
         super().__init__()
         if channels < 1:
             raise ValueError(f"HipGatedRecurrence needs at least one channel, got {channels}.")
-        if not rate > 0 or not math.isfinite(rate):
-            raise ValueError(f"`rate` has to be positive and finite, got {rate}.")
+        if not 0.0 < rate <= 2.0**126:
+            raise ValueError(f"`rate` has to be positive and at most 2^126, got {rate}.")
         if not 0.0 < fastest <= slowest < 1.0:
             raise ValueError(f"Expected 0 < fastest <= slowest < 1, got {fastest} and {slowest}.")
         self.channels, self.rate = int(channels), float(rate)
