@@ -167,6 +167,22 @@ def test_optimizer_options():
     assert opt.state_bits == 8 and opt.state_dict()["param_groups"][0]["state_bits"] == 8
 
 
+@pytest.mark.parametrize("options,message", [
+    ({"lr": -1.0}, "learning rate"), ({"betas": (0.9, 1.0)}, "betas"), ({"eps": -1.0}, "eps"), ({"state_bits": 32}, "same"),
+])
+def test_a_refused_group_is_not_added(options, message):
+    p, q = (torch.nn.Parameter(torch.zeros(4)) for _ in range(2))
+    opt = HipAdamW([p], state_bits=8)
+    with pytest.raises(ValueError, match=message):
+        opt.add_param_group({"params": [q], **options})
+    assert [g["params"] for g in opt.param_groups] == [[p]]
+    with pytest.raises(ValueError, match="32 or 8"):
+        HipAdamW([{"params": [q], "state_bits": 16}])
+    assert HipAdamW([{"params": [q], "state_bits": 8}]).state_bits == 8
+    opt.add_param_group({"params": [q], "lr": 0.5})
+    assert opt.param_groups[1]["lr"] == 0.5 and opt.param_groups[1]["state_bits"] == 8
+
+
 def test_module_decay_spans_the_asked_memory():
     module = HipGatedRecurrence(1000, rate=4.0, fastest=0.5, slowest=0.99)
     open_gate = torch.exp(-4.0 * torch.nn.functional.softplus(module.decay.detach().double()))

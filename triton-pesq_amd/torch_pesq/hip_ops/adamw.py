@@ -20,6 +20,8 @@ _NAMES = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_s
 
 
 def _check_options(group):
+    if group["state_bits"] not in _NAMES:
+        raise ValueError(f"`state_bits` has to be 32 or 8, got {group['state_bits']}.")
     lr, (beta1, beta2) = float(group["lr"]), group["betas"]
     if not (lr >= 0.0 and math.isfinite(lr)):
         raise ValueError(f"Invalid learning rate: {lr}")
@@ -46,12 +48,11 @@ class HipAdamW(torch.optim.Optimizer):
                                   "state_bits": int(state_bits)})
 
     def add_param_group(self, param_group):
-        super().add_param_group(param_group)
-        group = self.param_groups[-1]
-        _check_options(group)
-        if group["state_bits"] != self.param_groups[0]["state_bits"]:
-            del self.param_groups[-1]
+        options = {**self.defaults, **param_group}
+        _check_options(options)
+        if self.param_groups and options["state_bits"] != self.state_bits:
             raise ValueError("All parameter groups need the same `state_bits`.")
+        super().add_param_group(param_group)
         self._plan = None
 
     def __setstate__(self, state):
