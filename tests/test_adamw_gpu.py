@@ -337,6 +337,49 @@ def test_state_round_trip_and_torch_s_state():
     assert ours.param_groups[0]["lr"] == 1e-2
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_load_that_fails_changes_nothing(bits):
+    params = _params(torch.float32, seed=11, shapes=[(300,), (40, 40)])
+    twins = [torch.nn.Parameter(p.detach().clone()) for p in params]
+    opt, other = HipAdamW(params, state_bits=bits), HipAdamW(twins, state_bits=bits)
+
+    def step(seed, *optimizers):
+        for p, q, g in zip(params, twins, _grads(params, seed)):
+            p.grad, q.grad = g, g.clone()
+        for o in optimizers:
+            o.step()
+
+    step(80, opt, other)
+    held = copy.deepcopy(opt.state_dict())
+    bad = {
+        "other shape": lambda s: s["state"][1].update(exp_avg=s["state"][1]["exp_avg"][:2].clone()),
+        "other type": lambda s: s["state"][1].update(exp_avg_sq=s["state"][1]["exp_avg_sq"].double()),
+        "other names": lambda s: s["state"][1].update(momentum_buffer=s["state"][1]["exp_avg"]),
+        "no tensor": lambda s: s["state"][1].update(step="three"),
+        "no state": lambda s: s["state"].update({1: None}),
+        "no dictionary": lambda s: s.update(state=None),
+    }
+    for what, spoil in bad.items():
+        spoiled = copy.deepcopy(held)
+        for k in spoiled["state"]:
+            spoiled["state"][k]["exp_avg"].fill_(3)
+            spoiled["state"][k]["step"] = torch.tensor(77)
+        spoil(spoiled)
+        spoiled["param_groups"][0]["lr"] = 0.5
+        with pytest.raises(Exception) as error:
+            opt.load_state_dict(spoiled)
+        assert isinstance(error.value, (ValueError, TypeError, RuntimeError, AttributeError)), (what, error.value)
+        now = opt.state_dict()
+        assert now["param_groups"] == held["param_groups"], what
+        assert now["state"].keys() == held["state"].keys(), what
+        for k, of in held["state"].items():
+            assert all(torch.equal(torch.as_tensor(now["state"][k][name]).cpu(), t.cpu()) for name, t in of.items()), what
+    step(81, opt, other)
+    for p, q in zip(params, twins):
+        assert torch.equal(p, q) and opt.state[p]["step"] == 2
+        assert all(torch.equal(opt.state[p][name], other.state[q][name]) for name in opt.state[p])
+
+
 def test_group_added_later_keeps_the_moments():
     params = _params(torch.float32, seed=8, shapes=[(300,), (40, 40)])
     for bits in (32, 8):

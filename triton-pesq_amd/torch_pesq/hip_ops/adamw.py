@@ -65,12 +65,13 @@ class HipAdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def _build(self):
-        """Lay the moments of all parameters out, taking over what the state holds."""
+        """Lay the moments of all parameters out, taking over what the state holds.
+        A state that does not fit raises, and stays as it is."""
 
         bits = self.state_bits
         plan = _lib.torch_ext().AdamWPlan([list(group["params"]) for group in self.param_groups], bits)
         steps, index = plan.steps(), 0
-        copies = {}
+        laid_out, copies = [], {}
         for g, group in enumerate(self.param_groups):
             for k, p in enumerate(group["params"]):
                 views = dict(zip(_NAMES[bits], plan.views(g, k)), step=steps[index])
@@ -88,9 +89,10 @@ class HipAdamW(torch.optim.Optimizer):
                     to_all, held_all = copies.setdefault(to.dtype, ([], []))
                     to_all.append(to)
                     held_all.append(held)
-                self.state[p] = views
+                laid_out.append((p, views))
         for to_all, held_all in copies.values():
             torch._foreach_copy_(to_all, held_all)
+        self.state.update(laid_out)
         self._plan = plan
 
     def step(self, closure=None):
@@ -139,12 +141,12 @@ class HipAdamW(torch.optim.Optimizer):
                 raise ValueError(f"The loaded state has {group.get('state_bits', 32)} bits, expected {bits}.")
         params = {key: p for g, s in zip(groups, saved) for key, p in zip(s["params"], g["params"])}
         before = dict(self.state)
-        self.state.clear()
-        for key, held in state_dict["state"].items():
-            self.state[params[key]] = dict(held)
         try:
+            self.state.clear()
+            for key, held in state_dict["state"].items():
+                self.state[params[key]] = dict(held)
             self._build()
-        except ValueError:
+        except BaseException:
             self.state.clear()
             self.state.update(before)
             raise
