@@ -380,6 +380,29 @@ def test_a_load_that_fails_changes_nothing(bits):
         assert all(torch.equal(opt.state[p][name], other.state[q][name]) for name in opt.state[p])
 
 
+@pytest.mark.parametrize("theirs,message", [
+    (lambda p: torch.optim.AdamW(p, maximize=True), "maximize"),
+    (lambda p: torch.optim.AdamW(p, amsgrad=True), "amsgrad"),
+    (lambda p: torch.optim.Adam(p, weight_decay=0.1), "weight decay"),
+    (lambda p: torch.optim.Adam(p), None),
+])
+def test_states_of_optimizers_that_step_otherwise(theirs, message):
+    for stepped in (False, True):
+        params = _params(torch.float32, seed=12, shapes=[(40, 40)])
+        opt = theirs(params)
+        if stepped:
+            params[0].grad = _grads(params, 82)[0]
+            opt.step()
+        mine = HipAdamW(params, lr=0.25)
+        if message is None:
+            mine.load_state_dict(opt.state_dict())
+            assert mine.param_groups[0]["lr"] == 1e-3 and mine.param_groups[0]["weight_decay"] == 0
+            continue
+        with pytest.raises(ValueError, match=message):
+            mine.load_state_dict(opt.state_dict())
+        assert mine.param_groups[0]["lr"] == 0.25 and not mine.state
+
+
 def test_group_added_later_keeps_the_moments():
     params = _params(torch.float32, seed=8, shapes=[(300,), (40, 40)])
     for bits in (32, 8):

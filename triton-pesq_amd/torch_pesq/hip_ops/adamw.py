@@ -130,7 +130,9 @@ class HipAdamW(torch.optim.Optimizer):
         raise ValueError("The tensor is not one of the optimizer's parameters.")
 
     def load_state_dict(self, state_dict):
-        """Take over hyperparameters and moments; the moments keep their types."""
+        """Take over hyperparameters and moments; the moments keep their types.  States of
+        optimizers that step otherwise (``maximize``, ``amsgrad``, weight decay through
+        the gradients) are refused."""
 
         groups, saved = self.param_groups, state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
@@ -139,6 +141,11 @@ class HipAdamW(torch.optim.Optimizer):
         for group in saved:
             if group.get("state_bits", 32) != bits:
                 raise ValueError(f"The loaded state has {group.get('state_bits', 32)} bits, expected {bits}.")
+            for name in ("maximize", "amsgrad"):
+                if group.get(name):
+                    raise ValueError(f"The loaded state is of an optimizer with `{name}`, which HipAdamW has not.")
+            if group.get("decoupled_weight_decay") is False and group.get("weight_decay"):
+                raise ValueError("The loaded state's weight decay is part of its gradients; HipAdamW's is not.")
         params = {key: p for g, s in zip(groups, saved) for key, p in zip(s["params"], g["params"])}
         before = dict(self.state)
         try:
