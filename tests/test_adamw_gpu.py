@@ -403,6 +403,52 @@ def test_states_of_optimizers_that_step_otherwise(theirs, message):
         assert mine.param_groups[0]["lr"] == 0.25 and not mine.state
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_load_runs_the_hooks_and_takes_every_option(bits):
+    params = _params(torch.bfloat16, seed=13, shapes=[(300,), (40, 40)])
+    opt = HipAdamW([{"params": params[:1], "name": "first"}, {"params": params[1:], "lr": 0.5}], state_bits=bits)
+    for p, g in zip(params, _grads(params, 83)):
+        p.grad = g
+    opt.step()
+    held = copy.deepcopy(opt.state_dict())
+    held["param_groups"][1].update(max_lr=0.75, betas=[0.5, 0.25])
+
+    other = HipAdamW([{"params": params[:1]}, {"params": params[1:]}], state_bits=bits)
+    seen = []
+
+    def before(optimizer, state_dict):
+        seen.append(("before", len(optimizer.state)))
+        # an older name of the moments
+        state = {k: {n.replace("average", "exp_avg"): t for n, t in of.items()} for k, of in state_dict["state"].items()}
+        return dict(state_dict, state=state)
+
+    def after(optimizer):
+        seen.append(("after", [int(optimizer.state[p]["step"]) for p in params]))
+
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(after)
+    renamed = dict(held, state={k: {n.replace("exp_avg", "average"): t for n, t in of.items()}
+                                for k, of in held["state"].items()})
+    with pytest.raises(ValueError, match="bits"):
+        other.load_state_dict(dict(renamed, param_groups=[dict(g, state_bits=40 - bits) for g in held["param_groups"]]))
+    assert seen == [("before", 0)] and not other.state
+    other.load_state_dict(renamed)
+    assert seen == [("before", 0), ("before", 0), ("after", [1, 1])]
+    assert other.param_groups[0]["name"] == "first" and other.param_groups[1]["max_lr"] == 0.75
+    assert other.param_groups[1]["lr"] == 0.5 and tuple(other.param_groups[1]["betas"]) == (0.5, 0.25)
+    for k, p in enumerate(params):
+        assert all(torch.equal(other.state[p][n], torch.as_tensor(t)) for n, t in held["state"][k].items())
+        assert other.state[p]["exp_avg"].dtype == (torch.float32 if bits == 32 else torch.int8)
+    # back into torch's own, and from it
+    if bits == 32:
+        theirs = torch.optim.AdamW([{"params": params[:1]}, {"params": params[1:]}])
+        theirs.load_state_dict(other.state_dict())
+        other.load_state_dict(theirs.state_dict() | {"state": held["state"]})
+        assert other.param_groups[1]["lr"] == 0.5 and other.state_bits == 32
+    with pytest.raises(ValueError, match="learning rate"):
+        other.load_state_dict(dict(renamed, param_groups=[dict(g, lr=-1.0) for g in held["param_groups"]]))
+
+
 def test_group_added_later_keeps_the_moments():
     params = _params(torch.float32, seed=8, shapes=[(300,), (40, 40)])
     for bits in (32, 8):

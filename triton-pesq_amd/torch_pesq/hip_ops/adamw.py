@@ -18,6 +18,8 @@ __all__ = ["HipAdamW"]
 
 _NAMES = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
+_OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits")
+
 
 def _check_options(group):
     if group["state_bits"] not in _NAMES:
@@ -29,6 +31,14 @@ def _check_options(group):
         raise ValueError(f"Invalid betas, expected values in [0, 1): {group['betas']}")
     if not (group["eps"] >= 0.0 and group["weight_decay"] >= 0.0):
         raise ValueError(f"Invalid eps or weight decay: {group['eps']}, {group['weight_decay']}")
+
+
+class _Loaded:
+    """The state of one parameter on its way through torch's loading, which would
+    convert its tensors to the parameter's type."""
+
+    def __init__(self, held):
+        self.held = held
 
 
 class HipAdamW(torch.optim.Optimizer):
@@ -58,6 +68,11 @@ class HipAdamW(torch.optim.Optimizer):
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plan = None
+        loaded = [key for key, held in self.state.items() if isinstance(held, _Loaded)]
+        for key in loaded:
+            self.state[key] = self.state[key].held
+        if loaded:
+            self._build()
 
     @property
     def state_bits(self):
@@ -130,32 +145,37 @@ class HipAdamW(torch.optim.Optimizer):
         raise ValueError("The tensor is not one of the optimizer's parameters.")
 
     def load_state_dict(self, state_dict):
-        """Take over hyperparameters and moments; the moments keep their types.  States of
-        optimizers that step otherwise (``maximize``, ``amsgrad``, weight decay through
-        the gradients) are refused."""
+        """Take over options and moments as ``torch.optim.Optimizer`` does, hooks and
+        all; the moments keep their types.  States of optimizers that step otherwise
+        (``maximize``, ``amsgrad``, weight decay through the gradients) are refused.
+        A load that fails changes nothing."""
 
-        groups, saved = self.param_groups, state_dict["param_groups"]
-        if [len(g["params"]) for g in groups] != [len(g["params"]) for g in saved]:
-            raise ValueError("The loaded state has other parameter groups.")
-        bits = self.state_bits
-        for group in saved:
-            if group.get("state_bits", 32) != bits:
-                raise ValueError(f"The loaded state has {group.get('state_bits', 32)} bits, expected {bits}.")
-            for name in ("maximize", "amsgrad"):
-                if group.get(name):
-                    raise ValueError(f"The loaded state is of an optimizer with `{name}`, which HipAdamW has not.")
-            if group.get("decoupled_weight_decay") is False and group.get("weight_decay"):
-                raise ValueError("The loaded state's weight decay is part of its gradients; HipAdamW's is not.")
-        params = {key: p for g, s in zip(groups, saved) for key, p in zip(s["params"], g["params"])}
-        before = dict(self.state)
+        before = self.state, self.param_groups, self._plan
+        # (the last hook: it sees what the user's have made of the state)
+        handle = self.register_load_state_dict_pre_hook(HipAdamW._loadable)
         try:
-            self.state.clear()
-            for key, held in state_dict["state"].items():
-                self.state[params[key]] = dict(held)
-            self._build()
+            super().load_state_dict(state_dict)
         except BaseException:
-            self.state.clear()
-            self.state.update(before)
+            self.state, self.param_groups, self._plan = before
             raise
-        for group, held in zip(groups, saved):
-            group.update({k: v for k, v in held.items() if k in ("lr", "betas", "eps", "weight_decay", "initial_lr")})
+        finally:
+            handle.remove()
+
+    def _loadable(self, state_dict):
+        """The state as torch's loading takes it, after checks."""
+
+        groups, bits = [], self.state_bits
+        if [len(g["params"]) for g in self.param_groups] != [len(g["params"]) for g in state_dict["param_groups"]]:
+            raise ValueError("The loaded state has other parameter groups.")
+        for group, saved in zip(self.param_groups, state_dict["param_groups"]):
+            if saved.get("state_bits", 32) != bits:
+                raise ValueError(f"The loaded state has {saved.get('state_bits', 32)} bits, expected {bits}.")
+            for name in ("maximize", "amsgrad"):
+                if saved.get(name):
+                    raise ValueError(f"The loaded state is of an optimizer with `{name}`, which HipAdamW has not.")
+            if saved.get("decoupled_weight_decay") is False and saved.get("weight_decay"):
+                raise ValueError("The loaded state's weight decay is part of its gradients; HipAdamW's is not.")
+            groups.append({**{name: group[name] for name in _OPTIONS}, **saved})
+            _check_options(groups[-1])
+        state = {key: _Loaded(dict(held)) for key, held in state_dict["state"].items()}
+        return {**state_dict, "state": state, "param_groups": groups}
