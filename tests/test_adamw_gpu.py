@@ -6,6 +6,7 @@ values in a fixed order of operations, so a plain torch form in that order has
 to give the same codes and scales bit for bit.
 """
 
+import collections
 import copy
 import math
 
@@ -447,6 +448,92 @@ def test_load_runs_the_hooks_and_takes_every_option(bits):
         assert other.param_groups[1]["lr"] == 0.5 and other.state_bits == 32
     with pytest.raises(ValueError, match="learning rate"):
         other.load_state_dict(dict(renamed, param_groups=[dict(g, lr=-1.0) for g in held["param_groups"]]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_edits_of_state_and_groups_are_followed(bits):
+    """A cleared or replaced state, tensors put into it, and parameters put into or taken
+    out of a group count from the next step on, as in torch's optimizers."""
+
+    params = _params(torch.float32, seed=14, shapes=[(300,), (40, 40), (257,)])
+
+    def fresh(of):
+        return [torch.nn.Parameter(p.detach().clone()) for p in of]
+
+    def params_of(opt):
+        return opt.param_groups[0]["params"]
+
+    def step(opt, seed):
+        ps = params_of(opt)
+        for p, g in zip(ps, _grads(ps, seed)):
+            p.grad = g
+        opt.step()
+
+    def same(a, b):
+        for p, q in zip(params_of(a), params_of(b)):
+            assert torch.equal(p, q)
+            assert a.state[p].keys() == b.state[q].keys()
+            assert all(torch.equal(a.state[p][n], b.state[q][n]) for n in a.state[p])
+            assert all(torch.equal(x, y) for x, y in zip(a.moments(p), b.moments(q)))
+
+    def clear(opt):
+        opt.state.clear()
+
+    def replace(opt):
+        opt.state = collections.defaultdict(dict)
+
+    def delete(opt):
+        for p in params_of(opt):
+            del opt.state[p]
+
+    for forget in (clear, replace, delete):
+        opt = HipAdamW(fresh(params), state_bits=bits)
+        for seed in range(3):
+            step(opt, 90 + seed)
+        forget(opt)
+        again = HipAdamW(fresh(params_of(opt)), state_bits=bits)
+        for seed in range(2):
+            step(opt, 95 + seed)
+            step(again, 95 + seed)
+            same(opt, again)
+        assert len(opt.state_dict()["state"]) == 3
+
+    # a tensor of the state, a count, one parameter's whole state
+    for put in (lambda o, p: o.state[p].update(exp_avg=torch.zeros_like(o.state[p]["exp_avg"])),
+                lambda o, p: o.state[p].update(step=40),
+                lambda o, p: o.state.__setitem__(p, {})):
+        opt = HipAdamW(fresh(params), state_bits=bits)
+        step(opt, 100)
+        put(opt, params_of(opt)[0])
+        held = copy.deepcopy(opt.state_dict())
+        again = HipAdamW(fresh(params_of(opt)), state_bits=bits)
+        again.load_state_dict(held)
+        step(opt, 101)
+        step(again, 101)
+        same(opt, again)
+
+    # other parameters in the group
+    opt = HipAdamW(fresh(params), state_bits=bits)
+    step(opt, 110)
+    gone = params_of(opt)[1]
+    params_of(opt)[1] = torch.nn.Parameter(torch.ones(70, device="cuda"))
+    before = gone.detach().clone()
+    step(opt, 111)
+    assert torch.equal(gone, before)
+    assert [int(opt.state[p]["step"]) for p in params_of(opt)] == [2, 1, 2]
+    opt.param_groups[0]["params"] = params_of(opt)[:1]
+    step(opt, 112)
+    assert int(opt.state[params_of(opt)[0]]["step"]) == 3
+    # a tensor that does not fit is refused, and nothing has changed
+    p = params_of(opt)[0]
+    held, before = dict(opt.state[p]), p.detach().clone()
+    opt.state[p]["exp_avg"] = torch.zeros(5, device="cuda")
+    with pytest.raises(ValueError, match="exp_avg"):
+        step(opt, 113)
+    assert torch.equal(p, before)
+    opt.state[p]["exp_avg"] = held["exp_avg"]
+    step(opt, 113)
+    assert int(opt.state[p]["step"]) == 4
 
 
 def test_group_added_later_keeps_the_moments():

@@ -542,6 +542,61 @@ class AdamWPlan {
 
     at::Tensor steps() const { return steps_; }
 
+    // `state` and `groups` are what the plan stands for: see `current`.
+    void watch(const pybind11::dict &state, const pybind11::list &groups) {
+        entries_.clear();
+        params_.clear();
+        for (const auto &group : groups) {
+            params_.emplace_back();
+            for (const auto &p : pybind11::reinterpret_borrow<pybind11::dict>(group)["params"]) {
+                params_.back().push_back(pybind11::reinterpret_borrow<pybind11::object>(p));
+            }
+        }
+        for (const auto &[key, held] : state) {
+            Entry entry{pybind11::reinterpret_borrow<pybind11::object>(key),
+                        pybind11::reinterpret_borrow<pybind11::object>(held), {}};
+            if (PyDict_Check(held.ptr())) {
+                for (const auto &item : pybind11::reinterpret_borrow<pybind11::dict>(held)) {
+                    entry.values.push_back(pybind11::reinterpret_borrow<pybind11::object>(item.second));
+                }
+            }
+            entries_.push_back(std::move(entry));
+        }
+    }
+
+    // Whether the optimizer's state and groups are those that the plan was made
+    // from: by the identity of every entry, tensor and parameter, in order (through
+    // the interpreter's own interface: a few nanoseconds each, in every step).
+    bool current(const pybind11::dict &state, const pybind11::list &groups) const {
+        if (static_cast<size_t>(PyDict_Size(state.ptr())) != entries_.size() || groups.size() != params_.size()) {
+            return false;
+        }
+        static PyObject *const name = PyUnicode_InternFromString("params");
+        for (size_t g = 0; g < params_.size(); ++g) {
+            PyObject *group = PyList_GET_ITEM(groups.ptr(), static_cast<Py_ssize_t>(g));
+            PyObject *params = PyDict_Check(group) ? PyDict_GetItem(group, name) : nullptr;
+            if (!params || !PyList_Check(params)) return false;
+            if (static_cast<size_t>(PyList_GET_SIZE(params)) != params_[g].size()) return false;
+            for (size_t k = 0; k < params_[g].size(); ++k) {
+                if (PyList_GET_ITEM(params, static_cast<Py_ssize_t>(k)) != params_[g][k].ptr()) return false;
+            }
+        }
+        Py_ssize_t at = 0;
+        PyObject *key, *held, *value;
+        for (const Entry &entry : entries_) {
+            if (!PyDict_Next(state.ptr(), &at, &key, &held) || key != entry.key.ptr() || held != entry.held.ptr()) {
+                return false;
+            }
+            if (!PyDict_Check(held)) continue;
+            if (static_cast<size_t>(PyDict_Size(held)) != entry.values.size()) return false;
+            Py_ssize_t inner = 0;
+            for (const pybind11::object &kept : entry.values) {
+                if (!PyDict_Next(held, &inner, nullptr, &value) || value != kept.ptr()) return false;
+            }
+        }
+        return true;
+    }
+
     void step(int64_t group, double lr, double beta1, double beta2, double eps,
               double weight_decay) {
         struct Bucket {
@@ -616,6 +671,13 @@ class AdamWPlan {
     int64_t first(int64_t group, int64_t k) const { return first_.at(group).at(k); }
 
   private:
+    struct Entry {
+        pybind11::object key, held;
+        std::vector<pybind11::object> values;
+    };
+
+    std::vector<Entry> entries_;  // of the state
+    std::vector<std::vector<pybind11::object>> params_;
     std::vector<std::vector<at::Tensor>> groups_;
     int64_t bits_, total_ = 0, tensors_ = 0;
     std::vector<std::vector<int64_t>> first_, counts_;
@@ -653,5 +715,7 @@ void bind_network(pybind11::module_ &m) {
         .def("views", &AdamWPlan::views)
         .def("first", &AdamWPlan::first)
         .def("steps", &AdamWPlan::steps)
+        .def("watch", &AdamWPlan::watch)
+        .def("current", &AdamWPlan::current)
         .def("moments", &AdamWPlan::moments);
 }

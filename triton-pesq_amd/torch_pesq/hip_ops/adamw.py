@@ -108,7 +108,15 @@ class HipAdamW(torch.optim.Optimizer):
         for to_all, held_all in copies.values():
             torch._foreach_copy_(to_all, held_all)
         self.state.update(laid_out)
+        plan.watch(self.state, self.param_groups)
         self._plan = plan
+
+    def _current_plan(self):
+        """The plan, made again where groups or state were replaced, cleared or added to."""
+
+        if self._plan is None or not self._plan.current(self.state, self.param_groups):
+            self._build()
+        return self._plan
 
     def step(self, closure=None):
         """One step of all parameters that have a gradient, on the current stream."""
@@ -119,11 +127,10 @@ class HipAdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if self._plan is None:
-            self._build()
+        plan = self._current_plan()
         for g, group in enumerate(self.param_groups):
             beta1, beta2 = group["betas"]
-            self._plan.step(g, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"])
+            plan.step(g, float(group["lr"]), beta1, beta2, group["eps"], group["weight_decay"])
         return loss
 
     def moments(self, param=None):
@@ -132,15 +139,14 @@ class HipAdamW(torch.optim.Optimizer):
         the next multiple of 256 elements (zeros between).  With 32 bits these are
         the state itself, with 8 bits what its codes stand for."""
 
-        if self._plan is None:
-            self._build()
-        m, v = self._plan.moments() or (torch.zeros(0), torch.zeros(0))
+        plan = self._current_plan()
+        m, v = plan.moments() or (torch.zeros(0), torch.zeros(0))
         if param is None:
             return m, v
         for g, group in enumerate(self.param_groups):
             for k, p in enumerate(group["params"]):
                 if p is param:
-                    at = self._plan.first(g, k)
+                    at = plan.first(g, k)
                     return tuple(t[at : at + p.numel()].view(p.shape) for t in (m, v))
         raise ValueError("The tensor is not one of the optimizer's parameters.")
 
