@@ -617,6 +617,17 @@ int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
                     const pesq_adamw_options *options, void *exp_avg, void *exp_avg_sq,
                     float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream);
 
+/* The same with the tensors' numbers of steps kept in memory that the GPU reads and
+ * writes (options->step is not read): *steps[k] goes up by one when the work runs,
+ * so that each replay of a captured call is a step of its own.  Host memory has to
+ * be pinned; it holds the counts once the work is done.  `steps` is read before the
+ * call returns.  corrections: 2 count floats of scratch on the GPU, at a multiple of
+ * 8 bytes. */
+int pesq_adamw_step_counted(const pesq_adamw_tensor *tensors, int64_t count,
+                            const pesq_adamw_options *options, int64_t *const *steps,
+                            float *corrections, void *exp_avg, void *exp_avg_sq,
+                            float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream);
+
 /* The values that `count` (a multiple of 256) 8 bit moments stand for. */
 int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq, const float *exp_avg_scale,
                        const float *exp_avg_sq_scale, int64_t count, float *m, float *v,

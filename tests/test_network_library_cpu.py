@@ -220,6 +220,25 @@ def test_adamw_of_tensors_without_elements(bits):
     assert "null argument" in _message()
 
 
+def test_adamw_counted_steps_refuse():
+    """As the others, but for the number of the step, which is not theirs to give."""
+
+    lib, tensors = _lib.library(), (_lib.AdamwTensor * 1)(_lib.AdamwTensor(ANY, ANY, 100, 0))
+    good = {"dtype": 0, "state_bits": 32, "step": 0, "lr": 1e-3, "beta1": 0.9, "beta2": 0.999, "eps": 1e-8}
+    steps = (ctypes.c_void_p * 1)(ANY)
+
+    def call(count=1, steps=steps, corrections=ANY, arrays=(ANY, ANY, ANY, ANY), **changes):
+        return lib.pesq_adamw_step_counted(tensors, count, _lib.AdamwOptions(**dict(good, **changes)), steps,
+                                           corrections, *arrays, None)
+
+    for changes, message in (({"steps": None}, "null"), ({"corrections": None}, "null"), ({"corrections": ANY + 4}, "8 bytes"),
+                             ({"steps": (ctypes.c_void_p * 1)(None)}, "no count"), ({"beta1": 1.0}, "betas"),
+                             ({"arrays": (ANY, None, ANY, ANY)}, "null"), ({"count": -1}, "null")):
+        assert call(**changes) == 1 and message in _message(), changes
+    # nothing to do
+    assert call(count=0, steps=None, corrections=None) == 0
+
+
 def test_adamw_moments_fit_a_launch():
     """Work items of a launch, four elements each in whole workgroups, stay below 2^32."""
 

@@ -4,6 +4,8 @@ Each result is compared with the same call on small, contiguous, eager tensors,
 bit for bit: neither strides nor how the call is made may change it.
 """
 
+import copy
+
 import pytest
 import torch
 
@@ -160,6 +162,133 @@ def test_optimizer_step_in_a_graph():
         torch.cuda.synchronize()
         assert torch.equal(p, q)
         _same(captured.moments(), eager.moments())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_replays_of_a_captured_step_count(bits):
+    """Every replay is a step of its own: moments and counts as after as many eager
+    steps, and weights but for the corrections, which the GPU computes (one unit of
+    float32 in two factors of the update, 2^-22 of it a step).  Eager steps between
+    the replays count on, of other tensors too."""
+
+    lr, shapes = 1e-2, [(300,), (0,), (40, 40), (1025,)] + [(k % 7 + 1, 9) for k in range(120)]
+
+    def make():
+        g = torch.Generator().manual_seed(30)
+        params = [torch.nn.Parameter(torch.randn(s, generator=g).to(torch.bfloat16 if k % 5 == 4 else torch.float32).cuda())
+                  for k, s in enumerate(shapes)]
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        return params, HipAdamW([{"params": params[:2]}, {"params": params[2:], "weight_decay": 0.0}], lr=lr, state_bits=bits)
+
+    def fill(params, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        for p in params:
+            if p.grad is not None:
+                p.grad.copy_(torch.randn(p.shape, generator=g, device="cuda"))
+
+    (a, captured), (b, eager) = make(), make()
+    steps = 0
+
+    def check():
+        torch.cuda.synchronize()
+        _same(captured.moments(), eager.moments())
+        for p, q in zip(a, b):
+            assert int(captured.state[p]["step"]) == int(eager.state[q]["step"])
+            unit = 2.0**-8 if p.dtype == torch.bfloat16 else 2.0**-23
+            off = (p.detach().double() - q.detach().double()).abs()
+            # an update is below 10 lr here; a weight is rounded once a step on either side
+            assert (off <= steps * (2.0**-22 * 10 * lr + unit * (q.detach().double().abs() + 10 * lr))).all()
+
+    for seed in range(2):
+        fill(a, seed), fill(b, seed)
+        captured.step(), eager.step()
+        steps += 1
+    check()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        captured.step()
+    check()
+    for seed in range(2, 9):
+        fill(a, seed), fill(b, seed)
+        left = [(p, p.grad) for p in (a[2], b[2], a[7], b[7])]
+        if seed in (4, 7):
+            # an eager step, without two of the tensors
+            for p, _ in left:
+                p.grad = None
+            captured.step()
+        else:
+            graph.replay()
+        eager.step()
+        for p, grad in left:
+            p.grad = grad
+        steps += 1
+        check()
+    # the counts in a state are those of what was enqueued before
+    graph.replay()
+    eager.step()
+    steps += 1
+    held = captured.state_dict()
+    assert [int(of["step"]) for of in held["state"].values()] == [int(of["step"]) for of in eager.state_dict()["state"].values()]
+    check()
+    # a load reaches the graph
+    held = copy.deepcopy(held)
+    for _ in range(3):
+        graph.replay()
+    for p, q in zip(a, b):
+        p.data.copy_(q.data)
+    captured.load_state_dict(held)
+    for seed in range(20, 23):
+        fill(a, seed), fill(b, seed)
+        graph.replay()
+        eager.step()
+        steps += 1
+        check()
+    captured.state.clear()
+    assert captured.moments()[0].abs().max() == 0
+    again = HipAdamW([{"params": b[:2]}, {"params": b[2:], "weight_decay": 0.0}], lr=lr, state_bits=bits)
+    eager = again
+    for p, q in zip(a, b):
+        p.data.copy_(q.data)
+    for seed in range(30, 32):
+        fill(a, seed), fill(b, seed)
+        graph.replay()
+        eager.step()
+        steps += 1
+        check()
+    # a copy counts by itself
+    other = copy.deepcopy(captured)
+    for p, q in zip((p for g in other.param_groups for p in g["params"]), b):
+        p.grad = q.grad.clone()
+    other.step()
+    eager.step()
+    assert [int(of["step"]) for of in other.state.values()] == [3] * len(shapes)
+    _same(other.moments(), eager.moments())
+
+
+def test_what_a_graph_cannot_hold():
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+        p.grad = torch.ones_like(p)
+        opt = HipAdamW([p], state_bits=bits)
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="first step"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                opt.step()
+        opt.step()
+        torch.cuda.synchronize()
+        assert int(opt.state[p]["step"]) == 1 and (p < 1).all()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        opt.add_param_group({"params": [torch.nn.Parameter(torch.ones(4, device="cuda"))]})
+        with pytest.raises(RuntimeError, match="stay as they are"):
+            opt.step()
+        del opt.param_groups[1]
+        opt.step()
+        torch.cuda.synchronize()
+        assert int(opt.state[p]["step"]) == 2
 
 
 def test_streams_at_once():

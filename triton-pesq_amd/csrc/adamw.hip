@@ -31,9 +31,20 @@ namespace pesq {
 constexpr int kBlock = 256;  // elements per 8 bit scale
 constexpr float kSmallest = 0x1p-100f;
 
-struct AdamArgs {
-    float b1, c1, b2, c2, keep, step_size, correction, eps;
+// what of a step's factors depends on its number
+struct Corrections {
+    float step_size, root;
 };
+
+struct AdamArgs {
+    float b1, c1, b2, c2, keep, eps;
+    Corrections of_step;
+};
+
+__host__ __device__ inline Corrections corrections_of(double lr, double beta1, double beta2, double step) {
+    return {static_cast<float>(lr / (1.0 - pow(beta1, step))),
+            static_cast<float>(1.0 / sqrt(1.0 - pow(beta2, step)))};
+}
 
 // A launch takes up to kTensors tensors as kernel arguments: no table to copy to
 // the GPU, and new gradients each step cost nothing.  Workgroups go by tiles of
@@ -66,13 +77,15 @@ struct AdamList {
     void *m, *v;
     float *m_scale, *v_scale;
     AdamArgs args;
+    const Corrections *corrections;  // of each tensor where the GPU counts the steps, or NULL
 };
 static_assert(sizeof(AdamList) <= 4096, "kernel arguments");
 
 // as written: no contraction into fused multiply-adds
 #pragma clang fp contract(off)
 
-__device__ __forceinline__ float adamw(float p, float g, float &m, float &v, const AdamArgs &a) {
+__device__ __forceinline__ float adamw(float p, float g, float &m, float &v, const AdamArgs &a,
+                                       const Corrections &c) {
     m = m * a.b1 + g * a.c1;
     v = v * a.b2 + (g * g) * a.c2;
     // The hardware's root and reciprocal, each within one unit in the last place.
@@ -80,8 +93,8 @@ __device__ __forceinline__ float adamw(float p, float g, float &m, float &v, con
     // root flushes them, counts as 2^-120: with eps = 0 there is still a quotient.
     // (a NaN, as all of a block are whose scale is infinite, stays one)
     const float held = v < 0x1p-120f ? 0x1p-120f : v;
-    const float update = m * rcp_fast(__builtin_amdgcn_sqrtf(held) * a.correction + a.eps);
-    return p * a.keep - update * a.step_size;
+    const float update = m * rcp_fast(__builtin_amdgcn_sqrtf(held) * c.root + a.eps);
+    return p * a.keep - update * c.step_size;
 }
 
 // a lane's codes, and its moments in float32
@@ -228,6 +241,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     T *param = static_cast<T *>(t.param);
     const T *grad = static_cast<const T *>(t.grad);
     const AdamArgs a = list.args;
+    const Corrections c = list.corrections ? list.corrections[low] : a.of_step;
     const int64_t held = t.block + at / kBlock, mine = int64_t(t.block) * kRow + at / E;
     Lane<E> p, g, m, v;
     load_lane(param, at, count, p);
@@ -241,7 +255,7 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
     }
     // (past the end m, v and g are 0, and the moments stay 0)
 #pragma unroll
-    for (int k = 0; k < E; ++k) p.v[k] = adamw(p.v[k], g.v[k], m.v[k], v.v[k], a);
+    for (int k = 0; k < E; ++k) p.v[k] = adamw(p.v[k], g.v[k], m.v[k], v.v[k], a, c);
     store_lane(param, at, count, p);
     if constexpr (kEight) {
         const float sm = block_scale(m), sv = block_scale(v);
@@ -258,6 +272,22 @@ __global__ void __launch_bounds__(kAdamThreads) adamw_kernel(AdamList list) {
         static_cast<Lane<E> *>(list.m)[mine] = m;
         static_cast<Lane<E> *>(list.v)[mine] = v;
     }
+}
+
+// Counts of a launch's tensors that the GPU keeps, each up by one, and what follows
+// from them: a captured step's replays are steps of their own.
+struct CountList {
+    int64_t *steps[kTensors];
+    int count;
+    double lr, beta1, beta2;
+};
+
+__global__ void __launch_bounds__(kTensors) adamw_count_kernel(CountList list, Corrections *corrections) {
+    const int k = threadIdx.x;
+    if (k >= list.count) return;
+    const int64_t step = *list.steps[k] + 1;
+    *list.steps[k] = step;
+    corrections[k] = corrections_of(list.lr, list.beta1, list.beta2, static_cast<double>(step));
 }
 
 constexpr int kValues = 4;  // of a lane
@@ -290,14 +320,15 @@ using namespace pesq;
 
 static constexpr int64_t kMostTiles = (int64_t(1) << 32) / kAdamThreads - 1;  // workgroups of a launch
 
-extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
-                               const pesq_adamw_options *o, void *exp_avg, void *exp_avg_sq,
-                               float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
+// steps and corrections: of pesq_adamw_step_counted, or NULL
+static int adamw_step(const pesq_adamw_tensor *tensors, int64_t count, const pesq_adamw_options *o,
+                      int64_t *const *steps, Corrections *corrections, void *exp_avg, void *exp_avg_sq,
+                      float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
     PESQ_CHECK_ARG(o != nullptr && count >= 0 && (tensors || count == 0), "null argument");
     PESQ_CHECK_ARG(known_type(o->dtype), "unknown element type %d", int(o->dtype));
     PESQ_CHECK_ARG(o->state_bits == 32 || o->state_bits == 8, "moments have 32 or 8 bits, got %d",
                    int(o->state_bits));
-    PESQ_CHECK_ARG(o->step >= 1, "steps count from 1, got %lld", (long long)o->step);
+    PESQ_CHECK_ARG(steps || o->step >= 1, "steps count from 1, got %lld", (long long)o->step);
     PESQ_CHECK_ARG(o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0,
                    "betas have to be in [0, 1)");
     const bool eight = o->state_bits == 8;
@@ -313,13 +344,11 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
         PESQ_CHECK_ARG(tensors[k].count <= kMostTiles * tile && tensors[k].first < (int64_t(1) << 40),
                        "tensor %lld is too large", (long long)k);
     }
-    const double step = static_cast<double>(o->step);
     const AdamArgs a{static_cast<float>(o->beta1), static_cast<float>(1.0 - o->beta1),
                      static_cast<float>(o->beta2), static_cast<float>(1.0 - o->beta2),
                      static_cast<float>(1.0 - o->lr * o->weight_decay),
-                     static_cast<float>(o->lr / (1.0 - std::pow(o->beta1, step))),
-                     static_cast<float>(1.0 / std::sqrt(1.0 - std::pow(o->beta2, step))),
-                     static_cast<float>(o->eps)};
+                     static_cast<float>(o->eps),
+                     steps ? Corrections{} : corrections_of(o->lr, o->beta1, o->beta2, static_cast<double>(o->step))};
     AdamList list;
     list.count = 0;
     list.m = exp_avg;
@@ -327,26 +356,56 @@ extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
     list.m_scale = exp_avg_scale;
     list.v_scale = exp_avg_sq_scale;
     list.args = a;
+    list.corrections = corrections;
     int64_t tiles = 0;
+    const auto launch = [&](int64_t end) -> int {  // of the list, whose tensors are those before `end`
+        if (steps) {
+            CountList counts;
+            counts.count = list.count;
+            counts.lr = o->lr;
+            counts.beta1 = o->beta1;
+            counts.beta2 = o->beta2;
+            for (int k = 0; k < list.count; ++k) counts.steps[k] = steps[end - list.count + k];
+            adamw_count_kernel<<<1, kTensors, 0, stream>>>(counts, corrections + (end - list.count));
+            list.corrections = corrections + (end - list.count);
+        }
+        if (tiles > 0) launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
+        if (steps || tiles > 0) PESQ_CHECK_LAUNCH("pesq_adamw_step");
+        list.count = 0;
+        tiles = 0;
+        return PESQ_OK;
+    };
     for (int64_t k = 0; k < count; ++k) {
         const pesq_adamw_tensor &t = tensors[k];
-        if (t.count == 0) continue;
         const int64_t more = cdiv(t.count, tile);
         if (list.count == kTensors || tiles + more > kMostTiles) {
-            launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
-            PESQ_CHECK_LAUNCH("pesq_adamw_step");
-            list.count = 0;
-            tiles = 0;
+            if (int st = launch(k)) return st;
         }
+        // (one without elements has no tile, and is found by none)
         tiles += more;
         list.tensors[list.count++] = {t.param, t.grad, t.count, static_cast<uint32_t>(t.first / kBlock),
                                       static_cast<uint32_t>(tiles)};
     }
-    if (list.count > 0) {
-        launch_adamw(list, o->dtype, eight, static_cast<uint32_t>(tiles), stream);
-        PESQ_CHECK_LAUNCH("pesq_adamw_step");
-    }
-    return PESQ_OK;
+    return list.count > 0 ? launch(count) : PESQ_OK;
+}
+
+extern "C" int pesq_adamw_step(const pesq_adamw_tensor *tensors, int64_t count,
+                               const pesq_adamw_options *o, void *exp_avg, void *exp_avg_sq,
+                               float *exp_avg_scale, float *exp_avg_sq_scale, hipStream_t stream) {
+    return adamw_step(tensors, count, o, nullptr, nullptr, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale,
+                      stream);
+}
+
+extern "C" int pesq_adamw_step_counted(const pesq_adamw_tensor *tensors, int64_t count,
+                                       const pesq_adamw_options *o, int64_t *const *steps, float *corrections,
+                                       void *exp_avg, void *exp_avg_sq, float *exp_avg_scale,
+                                       float *exp_avg_sq_scale, hipStream_t stream) {
+    if (count == 0) return PESQ_OK;
+    PESQ_CHECK_ARG(count > 0 && steps && corrections, "null argument");
+    PESQ_CHECK_ARG(reinterpret_cast<uintptr_t>(corrections) % 8 == 0, "the corrections start at a multiple of 8 bytes");
+    for (int64_t k = 0; k < count; ++k) PESQ_CHECK_ARG(steps[k], "tensor %lld has no count", (long long)k);
+    return adamw_step(tensors, count, o, steps, reinterpret_cast<Corrections *>(corrections), exp_avg, exp_avg_sq,
+                      exp_avg_scale, exp_avg_sq_scale, stream);
 }
 
 extern "C" int pesq_adamw_moments(const void *exp_avg, const void *exp_avg_sq,

@@ -491,6 +491,13 @@ std::vector<at::Tensor> residual_norm(const at::Tensor &x, const OptTensor &bran
 
 // The parameters of one optimizer, the place of each in the moments' arrays,
 // and these arrays.  Gradients are taken from the parameters at each step.
+bool capturing(const c10::Device &device) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    const hipError_t error = hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()).stream(), &status);
+    TORCH_CHECK(error == hipSuccess, "hipStreamIsCapturing: ", hipGetErrorString(error));
+    return status != hipStreamCaptureStatusNone;
+}
+
 class AdamWPlan {
   public:
     static constexpr int64_t kBlock = 256;
@@ -513,8 +520,16 @@ class AdamWPlan {
                 ++tensors_;
             }
         }
-        steps_ = at::zeros({tensors_}, at::kLong);
-        if (tensors_ == 0) return;
+        if (tensors_ == 0) {
+            steps_ = at::zeros({0}, at::kLong);
+            return;
+        }
+        const c10::DeviceGuard guard(options.device());
+        TORCH_CHECK(!capturing(options.device()), "HipAdamW lays its moments out at its first step, which cannot be "
+                    "captured in a graph: take one before, or call `moments()`.");
+        // (pinned: the GPU counts in it once a step was captured)
+        steps_ = at::zeros({tensors_}, at::TensorOptions().dtype(at::kLong).pinned_memory(true));
+        corrections_ = at::empty({tensors_, 2}, options.dtype(at::kFloat));
         const auto type = [&](at::ScalarType t) { return options.dtype(t); };
         if (bits == 32) {
             arrays_ = {at::zeros({total_}, type(at::kFloat)), at::zeros({total_}, type(at::kFloat))};
@@ -568,19 +583,7 @@ class AdamWPlan {
     // from: by the identity of every entry, tensor and parameter, in order (through
     // the interpreter's own interface: a few nanoseconds each, in every step).
     bool current(const pybind11::dict &state, const pybind11::list &groups) const {
-        if (static_cast<size_t>(PyDict_Size(state.ptr())) != entries_.size() || groups.size() != params_.size()) {
-            return false;
-        }
-        static PyObject *const name = PyUnicode_InternFromString("params");
-        for (size_t g = 0; g < params_.size(); ++g) {
-            PyObject *group = PyList_GET_ITEM(groups.ptr(), static_cast<Py_ssize_t>(g));
-            PyObject *params = PyDict_Check(group) ? PyDict_GetItem(group, name) : nullptr;
-            if (!params || !PyList_Check(params)) return false;
-            if (static_cast<size_t>(PyList_GET_SIZE(params)) != params_[g].size()) return false;
-            for (size_t k = 0; k < params_[g].size(); ++k) {
-                if (PyList_GET_ITEM(params, static_cast<Py_ssize_t>(k)) != params_[g][k].ptr()) return false;
-            }
-        }
+        if (static_cast<size_t>(PyDict_Size(state.ptr())) != entries_.size() || !same_groups(groups)) return false;
         Py_ssize_t at = 0;
         PyObject *key, *held, *value;
         for (const Entry &entry : entries_) {
@@ -597,59 +600,90 @@ class AdamWPlan {
         return true;
     }
 
+    bool same_groups(const pybind11::list &groups) const {
+        if (groups.size() != params_.size()) return false;
+        static PyObject *const name = PyUnicode_InternFromString("params");
+        for (size_t g = 0; g < params_.size(); ++g) {
+            PyObject *group = PyList_GET_ITEM(groups.ptr(), static_cast<Py_ssize_t>(g));
+            PyObject *params = PyDict_Check(group) ? PyDict_GetItem(group, name) : nullptr;
+            if (!params || !PyList_Check(params)) return false;
+            if (static_cast<size_t>(PyList_GET_SIZE(params)) != params_[g].size()) return false;
+            for (size_t k = 0; k < params_[g].size(); ++k) {
+                if (PyList_GET_ITEM(params, static_cast<Py_ssize_t>(k)) != params_[g][k].ptr()) return false;
+            }
+        }
+        return true;
+    }
+
+    // Whether a step was captured in a graph.  From then on the GPU keeps the counts,
+    // the captured steps' and all others', and the plan's memory is the graph's.
+    bool captured() const { return captured_; }
+
     void step(int64_t group, double lr, double beta1, double beta2, double eps,
               double weight_decay) {
         struct Bucket {
             pesq_adamw_options options;
             std::vector<pesq_adamw_tensor> tensors;
+            std::vector<int64_t *> steps;
         };
-        std::vector<Bucket> buckets;  // parameters of one type and step count
+        std::vector<Bucket> buckets;  // parameters of one type and, where the host counts, step count
+        std::vector<size_t> stepped;
         std::vector<at::Tensor> copies;
         int64_t at_step = 0;
         for (int64_t g = 0; g < group; ++g) at_step += static_cast<int64_t>(groups_.at(g).size());
         int64_t *steps = steps_.data_ptr<int64_t>() + at_step;
         const auto &params = groups_.at(group);
+        const auto &firsts = first_[group], &counts = counts_[group];
+        const c10::Device device = tensors_ > 0 ? arrays_[0].device() : c10::Device(c10::kCPU);
+        if (tensors_ > 0 && !captured_) captured_ = capturing(device);
+        stepped.reserve(params.size());
         for (size_t k = 0; k < params.size(); ++k) {
-            const at::Tensor &p = params[k];
-            at::Tensor grad = p.grad();
+            const at::Tensor &p = params[k], &grad = p.grad();
             if (!grad.defined()) continue;
-            TORCH_CHECK(p.numel() == counts_[group][k] && p.is_contiguous() &&
-                            p.device() == arrays_[0].device(),
+            TORCH_CHECK(p.numel() == counts[k] && p.is_contiguous() && p.device() == device,
                         "HipAdamW needs contiguous parameters that keep their size and GPU.");
             TORCH_CHECK(grad.layout() == at::kStrided && grad.scalar_type() == p.scalar_type() &&
-                            grad.sizes() == p.sizes() && grad.device() == p.device(),
+                            grad.sizes() == p.sizes() && grad.device() == device,
                         "HipAdamW needs dense gradients of the parameters' type and GPU.");
-            if (!grad.is_contiguous()) {
-                grad = grad.contiguous();
-                copies.push_back(grad);
-            }
+            if (!grad.is_contiguous()) copies.push_back(grad.contiguous());
+            const void *from = (grad.is_contiguous() ? grad : copies.back()).data_ptr();
             const int32_t dtype = type_code(p, "a parameter");
             Bucket *bucket = nullptr;
             for (Bucket &b : buckets) {
-                if (b.options.dtype == dtype && b.options.step == steps[k] + 1) bucket = &b;
+                if (b.options.dtype == dtype && (captured_ || b.options.step == steps[k] + 1)) bucket = &b;
             }
             if (!bucket) {
-                buckets.push_back({{dtype, static_cast<int32_t>(bits_), steps[k] + 1, lr, beta1, beta2,
-                                    eps, weight_decay}, {}});
+                buckets.push_back({{dtype, static_cast<int32_t>(bits_), captured_ ? 0 : steps[k] + 1, lr, beta1,
+                                    beta2, eps, weight_decay}, {}, {}});
                 bucket = &buckets.back();
                 bucket->tensors.reserve(params.size());
             }
-            bucket->tensors.push_back({p.data_ptr(), grad.data_ptr(), p.numel(), first_[group][k]});
+            bucket->tensors.push_back({p.data_ptr(), from, counts[k], firsts[k]});
+            if (captured_) bucket->steps.push_back(steps + k);
+            stepped.push_back(k);
         }
         if (buckets.empty()) return;
         const c10::DeviceGuard guard(arrays_[0].device());
         const bool eight = bits_ == 8;
+        float *m_scale = eight ? arrays_[2].data_ptr<float>() : nullptr;
+        float *v_scale = eight ? arrays_[3].data_ptr<float>() : nullptr;
+        float *corrections = corrections_.data_ptr<float>() + 2 * at_step;
         for (const Bucket &b : buckets) {
-            check(pesq_adamw_step(b.tensors.data(), static_cast<int64_t>(b.tensors.size()), &b.options,
-                                  arrays_[0].data_ptr(), arrays_[1].data_ptr(),
-                                  eight ? arrays_[2].data_ptr<float>() : nullptr,
-                                  eight ? arrays_[3].data_ptr<float>() : nullptr,
-                                  current_stream(arrays_[0])),
-                  "pesq_adamw_step");
+            const int64_t count = static_cast<int64_t>(b.tensors.size());
+            if (captured_) {
+                check(pesq_adamw_step_counted(b.tensors.data(), count, &b.options, b.steps.data(), corrections,
+                                              arrays_[0].data_ptr(), arrays_[1].data_ptr(), m_scale, v_scale,
+                                              current_stream(arrays_[0])),
+                      "pesq_adamw_step_counted");
+                corrections += 2 * count;
+            } else {
+                check(pesq_adamw_step(b.tensors.data(), count, &b.options, arrays_[0].data_ptr(),
+                                      arrays_[1].data_ptr(), m_scale, v_scale, current_stream(arrays_[0])),
+                      "pesq_adamw_step");
+            }
         }
-        for (size_t k = 0; k < params.size(); ++k) {
-            if (!params[k].grad().defined()) continue;
-            ++steps[k];
+        for (const size_t k : stepped) {
+            if (!captured_) ++steps[k];
             written(params[k]);
         }
     }
@@ -681,8 +715,9 @@ class AdamWPlan {
     std::vector<std::vector<at::Tensor>> groups_;
     int64_t bits_, total_ = 0, tensors_ = 0;
     std::vector<std::vector<int64_t>> first_, counts_;
-    at::Tensor steps_;
+    at::Tensor steps_, corrections_;
     std::vector<at::Tensor> arrays_;
+    bool captured_ = false;
 };
 
 }  // namespace
@@ -717,5 +752,7 @@ void bind_network(pybind11::module_ &m) {
         .def("steps", &AdamWPlan::steps)
         .def("watch", &AdamWPlan::watch)
         .def("current", &AdamWPlan::current)
+        .def("same_groups", &AdamWPlan::same_groups)
+        .def("captured", &AdamWPlan::captured)
         .def("moments", &AdamWPlan::moments);
 }

@@ -296,6 +296,9 @@ SIGNATURES = {
     "pesq_adamw_step": (
         _INT, [ctypes.POINTER(AdamwTensor), _I64, ctypes.POINTER(AdamwOptions), _P, _P, _P, _P, _P],
     ),
+    "pesq_adamw_step_counted": (
+        _INT, [ctypes.POINTER(AdamwTensor), _I64, ctypes.POINTER(AdamwOptions), _P, _P, _P, _P, _P, _P, _P],
+    ),
     "pesq_adamw_moments": (_INT, [_P, _P, _P, _P, _I64, _P, _P, _P]),
 }
 

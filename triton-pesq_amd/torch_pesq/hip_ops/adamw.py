@@ -48,6 +48,12 @@ class HipAdamW(torch.optim.Optimizer):
     with dense gradients of their type; the step is computed in float32 and each
     parameter rounded once.  Parameters without a gradient are left as they are,
     and their count of steps with them.
+
+    A step that is not the first (``moments()`` prepares that) can be captured in a
+    HIP graph: each replay is a step of its own, with the options of the capture.
+    The GPU counts steps from then on; counts in the state are those of the work that
+    has been waited for, and ``state_dict()`` waits.  A load then changes the moments
+    that the graph works on; the groups have to stay as they are.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32):
@@ -63,16 +69,30 @@ class HipAdamW(torch.optim.Optimizer):
         if self.param_groups and options["state_bits"] != self.state_bits:
             raise ValueError("All parameter groups need the same `state_bits`.")
         super().add_param_group(param_group)
-        self._plan = None
+
+    def __getstate__(self):
+        self._settle()
+        return super().__getstate__()
 
     def __setstate__(self, state):
+        plan = self.__dict__.get("_plan")  # (none in a copy)
         super().__setstate__(state)
-        self._plan = None
+        self._plan = plan if plan is not None and plan.captured() else None
         loaded = [key for key, held in self.state.items() if isinstance(held, _Loaded)]
         for key in loaded:
             self.state[key] = self.state[key].held
-        if loaded:
+        if loaded or self._plan is not None:
             self._build()
+
+    def _settle(self):
+        """Wait for the counts that the GPU keeps."""
+
+        if self._plan is not None and self._plan.captured():
+            torch.cuda.synchronize(next(p.device for group in self.param_groups for p in group["params"]))
+
+    def state_dict(self):
+        self._settle()
+        return super().state_dict()
 
     @property
     def state_bits(self):
@@ -83,15 +103,29 @@ class HipAdamW(torch.optim.Optimizer):
         """Lay the moments of all parameters out, taking over what the state holds.
         A state that does not fit raises, and stays as it is."""
 
-        bits = self.state_bits
-        plan = _lib.torch_ext().AdamWPlan([list(group["params"]) for group in self.param_groups], bits)
+        bits, plan = self.state_bits, self._plan
+        in_place = plan is not None and plan.captured()
+        if in_place:
+            # a graph works on the plan's memory
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("The state of a HipAdamW cannot be replaced while a graph is captured.")
+            if not plan.same_groups(self.param_groups):
+                raise RuntimeError("The groups of a HipAdamW have to stay as they are once a step was captured.")
+            self._settle()
+        else:
+            plan = _lib.torch_ext().AdamWPlan([list(group["params"]) for group in self.param_groups], bits)
         steps, index = plan.steps(), 0
         laid_out, copies = [], {}
         for g, group in enumerate(self.param_groups):
             for k, p in enumerate(group["params"]):
                 views = dict(zip(_NAMES[bits], plan.views(g, k)), step=steps[index])
                 index += 1
-                for name, held in self.state.get(p, {}).items():
+                state = self.state.get(p, {})
+                if in_place:
+                    # (what is not there starts again; what is may be a view of what is written)
+                    state = {name: torch.as_tensor(t).clone() for name, t in state.items()}
+                    state = {**{name: torch.zeros_like(t) for name, t in views.items()}, **state}
+                for name, held in state.items():
                     if name not in views:
                         raise ValueError(f"A state of {bits} bits has no `{name}`.")
                     held = torch.as_tensor(held)
