@@ -521,6 +521,9 @@ int pesq_epilogue_backward(const float *d_symm, const float *d_asymm, const floa
  * to each other.  decay [channels], initial [batch, channels] (NULL = 0) and
  * reset [batch, time] (NULL = none) are contiguous.  At most 65535 batch
  * items, 2^24 channels and 2^32 steps, which start less than 2^27 bytes apart.
+ * Workgroups of a row wait for each other's results; a wait that had no answer
+ * for seconds (the GPU did not run its other workgroups) gives up, and the results
+ * after it are NaN: no status reports that.
  * No counterpart in the reference. */
 typedef struct pesq_recurrence {
     int64_t batch, time, channels;

@@ -25,10 +25,11 @@
 //      runs its steps again, from registers.
 //
 // Every kFan chunks the last one also publishes the pair of all of them, so a
-// chunk folds at most time / (kFan chunk) + kFan - 1 pairs, and never waits for
-// another's state, only for pairs, which need none: the depth is three memory
-// round trips whatever the length.  The order of the folds is fixed: results do
-// not depend on which workgroup was first.
+// chunk folds at most time / (kFan chunk) + kFan - 1 pairs, kRound between two
+// barriers, and never waits for another's state, only for pairs, which need none:
+// three memory round trips deep however long the row, while the pairs to fold grow
+// with it (64000 steps: 250 chunks, 30 pairs for the last one).  The order of the
+// folds is fixed: results do not depend on which workgroup was first.
 //
 // A published pair is one 64 bit word, written and read by relaxed device scope
 // atomics and valid by itself (kPending, which a fill kernel writes, is a NaN no
@@ -422,9 +423,10 @@ __device__ __forceinline__ void for_part(int left, Body body) {
     }
 }
 
-// Bound by memory and by waiting: 16 x 3751 x 960 bfloat16 takes 128 us, 3.8 TB/s,
-// where the same moves alone take 103.  Five wavefronts a SIMD (96 registers, one
-// spilled) hide more of the waits: 142 us with the four that 97 registers leave.
+// Bound by memory and by waiting: 16 x 3751 x 960 bfloat16 takes 134 us (median; 125
+// to 146 by run and card), 3.5 TB/s, where the same moves alone took 103.  Five
+// wavefronts a SIMD (96 registers, one spilled) hide more of the waits: 128 us against
+// 142 us with the four that 97 registers leave, on one card.
 template <class T, bool kReset>
 __global__ void __launch_bounds__(kMaxWaves *kWave, 5)
     recurrence_fwd_kernel(RecArgs p, T *y, float *last, float *starts, uint64_t *words) {
@@ -475,8 +477,8 @@ __global__ void __launch_bounds__(kMaxWaves *kWave, 5)
     }
 }
 
-// 16 x 3751 x 960 bfloat16: 209 us, 4.0 TB/s, where the same moves alone take 173
-// and the vector units issue for 136.
+// 16 x 3751 x 960 bfloat16: 216 us (median; 201 to 234 by run and card), 3.8 TB/s,
+// where the same moves alone took 173 and the vector units issue for 136.
 //
 // G as a carry c between steps: g = dy + c, c = a g (0 at a reset), from the
 // last step to the first; chunk 0 of the fold is the last in time.
@@ -647,8 +649,12 @@ static Plan plan_of(const pesq_recurrence *p) {
     const int64_t parts = cdiv(p->time, kSteps);
     // Few wavefronts leave room for several workgroups on a compute unit, of which
     // some compute while others wait (16 x 3751 x 960 bfloat16, forward and backward:
-    // 356 us with 4, 380 us with 8); many keep the chunks of a long row few
-    // (1 x 64000 x 65 float16: 78 us with 16, 103 us with half as many steps each).
+    // 356 us with 4, 380 us with 8); many keep the chunks of a long row, and the pairs
+    // to fold, few.  Forward and backward in bfloat16, with 16 / with 4:
+    //   1 x 64000 x 65    75 /  98 us      2 x 120000 x 256   448 / 579 us
+    //   1 x 64000 x 512  242 / 275 us      4 x 32000 x 512    453 / 465 us
+    //   8 x 20000 x 1024  1055 / 1033 us   16 x 17000 x 512   905 / 876 us
+    // so the length decides, and rows just past kLongRow in large batches lose 2 to 3 %.
     const int most = parts / kWaves > kLongRow ? kMaxWaves : kWaves;
     plan.waves = parts < most ? static_cast<int>(parts < 1 ? 1 : parts) : most;
     plan.chunks = parts < 1 ? 1 : cdiv(parts, plan.waves);

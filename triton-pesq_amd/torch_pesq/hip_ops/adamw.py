@@ -53,7 +53,8 @@ class HipAdamW(torch.optim.Optimizer):
     HIP graph: each replay is a step of its own, with the options of the capture.
     The GPU counts steps from then on; counts in the state are those of the work that
     has been waited for, and ``state_dict()`` waits.  A load then changes the moments
-    that the graph works on; the groups have to stay as they are.
+    that the graph works on, and so does an edit of the state, from the next
+    ``moments()`` or eager step on; the groups have to stay as they are.
     """
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *, state_bits=32):
