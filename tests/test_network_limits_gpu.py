@@ -267,6 +267,26 @@ def test_replays_of_a_captured_step_count(bits):
     _same(other.moments(), eager.moments())
 
 
+def test_counts_outlive_their_optimizer():
+    """Replays that are still to run when the optimizer goes count in memory that no
+    other pinned tensor gets."""
+
+    p = torch.nn.Parameter(torch.ones(2**24, device="cuda"))
+    p.grad = torch.ones_like(p)
+    opt = HipAdamW([p])
+    opt.moments()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for _ in range(200):
+        graph.replay()
+    del opt
+    others = [torch.zeros(1, dtype=torch.int64, pin_memory=True) for _ in range(20)]
+    torch.cuda.synchronize()
+    assert all(int(t) == 0 for t in others)
+
+
 def test_what_a_graph_cannot_hold():
     for bits in (32, 8):
         p = torch.nn.Parameter(torch.ones(300, device="cuda"))

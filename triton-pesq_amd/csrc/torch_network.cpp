@@ -494,6 +494,10 @@ std::vector<at::Tensor> residual_norm(const at::Tensor &x, const OptTensor &bran
 bool capturing(const c10::Device &device) {
     hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
     const hipError_t error = hipStreamIsCapturing(c10::hip::getCurrentHIPStream(device.index()).stream(), &status);
+    if (error == hipErrorStreamCaptureImplicit) {  // the default stream, while another one is captured
+        (void)hipGetLastError();
+        return false;
+    }
     TORCH_CHECK(error == hipSuccess, "hipStreamIsCapturing: ", hipGetErrorString(error));
     return status != hipStreamCaptureStatusNone;
 }
@@ -635,7 +639,12 @@ class AdamWPlan {
         const auto &params = groups_.at(group);
         const auto &firsts = first_[group], &counts = counts_[group];
         const c10::Device device = tensors_ > 0 ? arrays_[0].device() : c10::Device(c10::kCPU);
-        if (tensors_ > 0 && !captured_) captured_ = capturing(device);
+        if (tensors_ > 0 && !captured_ && capturing(device)) {
+            captured_ = true;
+            // A graph may count after the optimizer is gone, and nothing tells the allocator of pinned
+            // memory: the counts stay where they are until the process ends.
+            new at::Tensor(steps_);
+        }
         stepped.reserve(params.size());
         for (size_t k = 0; k < params.size(); ++k) {
             const at::Tensor &p = params[k], &grad = p.grad();
