@@ -285,8 +285,9 @@ struct CountList {
 __global__ void __launch_bounds__(kTensors) adamw_count_kernel(CountList list, Corrections *corrections) {
     const int k = threadIdx.x;
     if (k >= list.count) return;
-    const int64_t step = *list.steps[k] + 1;
-    *list.steps[k] = step;
+    // (past the GPU's caches: the host writes there between launches)
+    const int64_t step = __hip_atomic_load(list.steps[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM) + 1;
+    __hip_atomic_store(list.steps[k], step, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     corrections[k] = corrections_of(list.lr, list.beta1, list.beta2, static_cast<double>(step));
 }
 

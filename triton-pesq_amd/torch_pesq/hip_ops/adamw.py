@@ -17,7 +17,6 @@ from .. import _lib
 __all__ = ["HipAdamW"]
 
 _NAMES = {32: ("exp_avg", "exp_avg_sq"), 8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
-
 _OPTIONS = ("lr", "betas", "eps", "weight_decay", "state_bits")
 
 
